@@ -117,7 +117,7 @@ def run(s):
 
     # the error of the logits, in units of 2^-30, narrowed to 2^-7
     n = torch.frexp(S.double()).exponent.long() - 32
-    p = ((_exp_weights(M - acc, e) * ((1 << 62) // (S >> n))) >> 32) >> (n - 2)
+    p = ((_exp_weights(M - acc, e) * (((1 << 63) - 1) // (S >> n))) >> 32) >> (n - 3)
     p = p * used.any(1, keepdim=True)
     p.scatter_add_(1, at, -((share << 30) // share.sum(1, keepdim=True).clamp(min=1)) * used)
     four = (c["vocab"] + 3) // 4 * 4
