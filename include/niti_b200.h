@@ -496,6 +496,50 @@ NITI_API int niti_fc_head_supported(int B, int F, int J);
 NITI_API size_t niti_fc_head_scratch_bytes(int B, int F, int J);
 NITI_API int niti_fc_head_train_i8(const niti_fc_head_args* args, void* stream);
 
+/* ---------------------------------------------------------------- a vocabulary of classes
+ * TiLinear.forward + TiLoss.forward + TiLinear.backward (ti_torch.py:241-266, ti_loss.py:6-36) for a last layer with so many
+ * classes that its logits should not be kept: the vocabulary is taken in pieces and only the wanted classes' logits, a maximum
+ * and a sum per 64 classes and (for training) a bounded piece of int8 errors pass through scratch.  The softmax works on the
+ * int32 accumulators, not on logits narrowed to int8, and has 30 bits instead of TiLoss' 11, whose errors are all zero for
+ * 2048 equal classes.  Integers throughout, in a fixed definition (vocab_kernels.cu), so results do not depend on how the
+ * work is split.
+ *   x [T][F] int8 with *exp_x; w [V][F] int8 with *exp_w; logits are sum_f x w * 2^(*exp_x + *exp_w).
+ *   top == null (cross entropy): entries == 1, index int64 [T] = the wanted class of each row; ignore_index: rows to leave out.
+ *   top != null (distillation): index int64 [T][entries], the classes of a teacher's `entries` largest logits (any order,
+ *     negative: no entry, a class listed twice counts twice), top [T][entries] those logits, int8 or (top_is_int32) int32, with
+ *     *exp_top.  The teacher's distribution is the softmax over the row's entries, the student's over the vocabulary, both at
+ *     temperature 2^temperature_log2 (0 for cross entropy).
+ *   loss float32 [T]: -ln p[index], or 4^temperature_log2 * sum_k q_k (ln q_k - ln p[index_k]).  0 for rows that are left out or
+ *     have no entry, NaN where a class is not below V (or negative and not ignore_index); these rows have no error.
+ * With g32 != null the gradients of the sum of the losses too (e8, exp_err, g32 and grad_maxabs are then required):
+ *   err8 = p - q narrowed to int8 in units of 2^-7 by loss_round (a row of round_up(V, 4) random words of stream loss_stream per
+ *     token where it is stochastic); what err_round, bits and err_stream say narrows the int32 error err8 W to e8 [T][F] as
+ *     err_calc does (ti_torch.py:119-133), *exp_err = shift + *exp_w - 7 + temperature_log2;
+ *   g32 [V][F] = err8^T x, *grad_maxabs = max |g32|, for niti_update_i8.
+ *   sample_offset: global index of the first row, for the random words.
+ * scratch: niti_vocab_scratch_bytes(T, F, V, entries, g32 != null) bytes, 16-byte aligned, contents irrelevant.  T, F < 2^17,
+ * V <= 2^18, entries <= 128 (niti_vocab_supported), any F (rows of other lengths than multiples of 16 go through copies).  x, w,
+ * e8 and g32 16-byte aligned.  Calls on different streams need scratch of their own. */
+typedef struct niti_vocab_args {
+    const int8_t* x; const int32_t* exp_x;
+    const int8_t* w; const int32_t* exp_w;
+    const int64_t* index; int64_t ignore_index;
+    const void* top; const int32_t* exp_top;
+    float* loss;
+    int8_t* e8; int32_t* exp_err;
+    int32_t* g32; uint32_t* grad_maxabs;
+    void* scratch; size_t scratch_bytes;
+    int32_t T, F, V, entries, top_is_int32, temperature_log2;
+    int32_t bits, loss_round, err_round;
+    uint32_t loss_stream, err_stream;
+    const uint64_t* seed;
+    uint64_t sample_offset;
+    int32_t* status;
+} niti_vocab_args;
+NITI_API int niti_vocab_supported(int T, int F, int V, int entries);
+NITI_API size_t niti_vocab_scratch_bytes(int T, int F, int V, int entries, int train);
+NITI_API int niti_vocab_loss_i8(const niti_vocab_args* args, void* stream);
+
 /* TiFloatToInt8 + the NCHW -> NHWC permute of TiNet.forward (ti_torch.py:341-356, ti_net.py:18-19):
  * x f32 [N][C][H][W] -> x8 int8 [N][H][W][C], *exp_out = ceil(log2(max|x|)) - 7.
  * `scratch` is one uint32 word (cleared by the call). */

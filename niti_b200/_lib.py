@@ -76,6 +76,9 @@ SIGNATURES = {
     "niti_fc_head_supported": (_i, [_i, _i, _i]),
     "niti_fc_head_scratch_bytes": (_sz, [_i, _i, _i]),
     "niti_fc_head_train_i8": (_i, [_p, _p]),
+    "niti_vocab_supported": (_i, [_i] * 4),
+    "niti_vocab_scratch_bytes": (_sz, [_i] * 5),
+    "niti_vocab_loss_i8": (_i, [_p, _p]),
     "niti_dp_exchange_bytes": (_sz, []),
     "niti_peer_copy": (_i, [_p, _p, _sz, _p]),
     "niti_peer_arena_create": (_i, [_sz, _p, _p]),
@@ -106,6 +109,14 @@ class DpUpdateArgs(C.Structure):
     _fields_ = [("items", _p), ("count", C.c_int32), ("rank", C.c_int32), ("world", C.c_int32),
                 ("weights", _p), ("grads", _p), ("exchange", _p), ("mu", C.c_int32), ("round_mode", C.c_int32),
                 ("seed", _p), ("maxabs", _p), ("status", _p)]
+
+
+class VocabArgs(C.Structure):
+    """niti_vocab_args of include/niti_b200.h"""
+    _fields_ = ([("x", _p), ("exp_x", _p), ("w", _p), ("exp_w", _p), ("index", _p), ("ignore_index", _i64), ("top", _p), ("exp_top", _p),
+                 ("loss", _p), ("e8", _p), ("exp_err", _p), ("g32", _p), ("grad_maxabs", _p), ("scratch", _p), ("scratch_bytes", _sz)] +
+                [(n, C.c_int32) for n in ("T", "F", "V", "entries", "top_is_int32", "temperature_log2", "bits", "loss_round", "err_round")] +
+                [("loss_stream", _u32), ("err_stream", _u32), ("seed", _p), ("sample_offset", _u64), ("status", _p)])
 
 
 class FcHeadArgs(C.Structure):

@@ -15,7 +15,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libniti_b200.so")
 OPS = os.path.join(PKG, "_torch_ops.so")
-SOURCES = ["api.cu", "umma_kernels.cu", "simt_kernels.cu", "head_kernels.cu"]
+SOURCES = ["api.cu", "umma_kernels.cu", "simt_kernels.cu", "head_kernels.cu", "vocab_kernels.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
 

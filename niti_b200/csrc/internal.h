@@ -41,9 +41,13 @@ extern int g_stage_cap;  // experiments: cap on the shared-memory stages the GEM
 
 // tensor-core (tcgen05) paths, umma_kernels.cu; `out` is int32 (fused == null) or int8
 int umma_gemm_splits(int M, int N, int K);
+struct GemmExtra {
+    int ldb;         // row pitch of B in elements (0: dense)
+    int accumulate;  // 1: an int32 result is added to what is there (by TMA reductions), the splits of the reduction too; no maximum
+};
 int umma_gemm(const int8_t* A, const int8_t* B, void* out, unsigned* maxabs, int M, int N, int K, int trans_a,
               int trans_b, int splits, const FusedArgs* fused, int32_t* status, cudaStream_t st, int rows32 = 0,
-              int lda = 0, int ldc = 0);  // row pitches of A and of an int32 result in elements (0: dense)
+              int lda = 0, int ldc = 0, const GemmExtra* more = nullptr);  // row pitches of A and of an int32 result in elements (0: dense)
 int umma_conv(const int8_t* x, const int8_t* w, void* out, unsigned* maxabs, int Nimg, int H, int W, int C, int K,
               int R, int S, int pad, int flip, const FusedArgs* fused, int32_t* status, cudaStream_t st);
 // red / outc: reduction channels per tap, output channels; k3: 3x3 filters, padding 1

@@ -592,6 +592,66 @@ PyObject* loss_err(Args& a) {
     }
     return wrap(err);
 }
+// A vocabulary's losses: arguments x, exp_x, w, exp_w, index, ignore_index, top, exp_top, temperature_log2, train and, where that is
+// true, bits, loss_mode, err_mode, seed, loss_stream, err_stream, sample_offset, g32.
+PyObject* vocab_loss(Args& a) {
+    const Tensor &x = a.tensor(), &exp_x = a.tensor(), &w = a.tensor(), &exp_w = a.tensor(), &index = a.tensor();
+    niti_vocab_args v{};
+    v.ignore_index = a.integer();
+    const Tensor *top = a.maybe(), *exp_top = a.maybe();
+    const int64_t temperature = a.integer();
+    const bool train = a.flag();
+    const Tensor *seed = nullptr, *g32 = nullptr;
+    if (train) {
+        v.bits = a.i32(); v.loss_round = a.i32(); v.err_round = a.i32();
+        seed = a.maybe();
+        v.loss_stream = a.u32(); v.err_stream = a.u32(); v.sample_offset = a.u64();
+        g32 = a.maybe();
+    }
+    need_cuda({&x, &exp_x, &w, &exp_w, &index, top, exp_top, seed, g32});
+    for (const Tensor* t : {&exp_x, &w, &exp_w, &index, top, exp_top, seed, g32})
+        TORCH_CHECK(t == nullptr || t->device() == x.device(), "niti_b200 vocab ops: tensors on different devices");
+    TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.scalar_type() == at::kChar && w.scalar_type() == at::kChar && x.size(1) == w.size(1),
+                "niti_b200 vocab ops: x int8 [tokens, features] and w int8 [classes, features] were expected");
+    for (const Tensor* t : {&exp_x, &exp_w, exp_top})
+        TORCH_CHECK(t == nullptr || (t->scalar_type() == at::kInt && t->numel() == 1), "niti_b200 vocab ops: an exponent is one int32");
+    TORCH_CHECK(index.scalar_type() == at::kLong && (top ? index.dim() == 2 : index.dim() == 1) && index.size(0) == x.size(0),
+                "niti_b200 vocab ops: classes are int64, [tokens] or with a teacher [tokens, entries]");
+    TORCH_CHECK((top == nullptr) == (exp_top == nullptr) && (top == nullptr || (top->sizes() == index.sizes() && (top->scalar_type() == at::kChar || top->scalar_type() == at::kInt))),
+                "niti_b200 vocab ops: a teacher's logits are int8 or int32, one to each class, with an exponent");
+    TORCH_CHECK(temperature >= -30 && temperature <= 30, "niti_b200 vocab ops: the temperature's exponent lies between -30 and 30");
+    TORCH_CHECK(seed == nullptr || (seed->scalar_type() == at::kLong && seed->numel() >= 1), "niti_b200 vocab ops: the seed is one int64");
+    TORCH_CHECK(g32 == nullptr || (g32->scalar_type() == at::kInt && g32->sizes() == w.sizes()), "niti_b200 vocab ops: g32 is int32 of the weights' shape");
+    const int64_t T = x.size(0), F = x.size(1), V = w.size(0), K = top ? index.size(1) : 1;
+    TORCH_CHECK(T < (1ll << 31) && F < (1ll << 31) && V < (1ll << 31) && K < (1ll << 31) && niti_vocab_supported(int(T), int(F), int(V), int(K)),
+                "niti_b200 vocab ops: 1 to 131071 tokens and features, 1 to 262144 classes and 1 to 128 entries are supported: got ", T, ", ", F, ", ", V, ", ", K);
+    Tensor loss, e8, exp_err, gmax, g;
+    {
+        Launch l(x);
+        const auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; };
+        const Tensor xa = F % 16 != 0 || aligned(x) ? x : x.clone(), wa = F % 16 != 0 || aligned(w) ? w : w.clone();
+        loss = l.empty({T}, at::kFloat);
+        v.x = cptr<int8_t>(xa); v.exp_x = cptr<int32_t>(exp_x); v.w = cptr<int8_t>(wa); v.exp_w = cptr<int32_t>(exp_w);
+        v.index = cptr<int64_t>(index); v.top = cptr(top); v.exp_top = cptr<int32_t>(exp_top); v.loss = mptr<float>(loss);
+        v.T = int(T); v.F = int(F); v.V = int(V); v.entries = int(K);
+        v.top_is_int32 = top != nullptr && top->scalar_type() == at::kInt; v.temperature_log2 = int(temperature);
+        if (train) {
+            e8 = l.empty({T, F}, at::kChar);
+            std::pair<Tensor, Tensor> e = two_words(l);
+            exp_err = e.first;
+            gmax = l.empty({1}, at::kInt);
+            g = g32 ? *g32 : l.empty({V, F}, at::kInt);
+            v.e8 = mptr<int8_t>(e8); v.exp_err = mptr<int32_t>(exp_err); v.g32 = mptr<int32_t>(g); v.grad_maxabs = mptr<uint32_t>(gmax);
+            v.seed = cptr<uint64_t>(seed);
+        }
+        v.scratch_bytes = niti_vocab_scratch_bytes(v.T, v.F, v.V, v.entries, train);
+        const Tensor scratch = l.bytes(v.scratch_bytes);
+        v.scratch = mptr(scratch);
+        v.status = l.status();
+        check(niti_vocab_loss_i8(&v, l.stream), "niti_vocab_loss_i8");
+    }
+    return train ? tuple(loss, e8, exp_err, g, gmax) : wrap(loss);
+}
 PyObject* update(Args& a) {
     const Tensor &w = a.tensor(), &g32 = a.tensor(), &maxabs = a.tensor();
     const int mu = a.i32(), mode = a.i32();
@@ -658,7 +718,7 @@ PyMethodDef methods[] = {
     NITI_ENTRY(conv_wgrad_batch_inner_supported), NITI_ENTRY(conv_wgrad_batch_inner), NITI_ENTRY(maxpool_bwd_f16),
     NITI_ENTRY(conv_wgrad_from_patches), NITI_ENTRY(conv_wgrad_update), NITI_ENTRY(conv_wgrad_accumulate), NITI_ENTRY(gemm_acc), NITI_ENTRY(requant),
     NITI_ENTRY(absmax), NITI_ENTRY(maxpool_fwd), NITI_ENTRY(maxpool_bwd), NITI_ENTRY(relu_fwd), NITI_ENTRY(relu_bwd),
-    NITI_ENTRY(dropout), NITI_ENTRY(loss_err), NITI_ENTRY(update), NITI_ENTRY(quantize_input), NITI_ENTRY(publish_step),
+    NITI_ENTRY(dropout), NITI_ENTRY(loss_err), NITI_ENTRY(vocab_loss), NITI_ENTRY(update), NITI_ENTRY(quantize_input), NITI_ENTRY(publish_step),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_torch_ops", "native torch front end of libniti_b200 (" NITI_OPS_TAG ")", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

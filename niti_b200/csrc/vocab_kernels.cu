@@ -1,0 +1,650 @@
+// A last layer with a vocabulary of classes and the losses over it: softmax cross entropy against one class a row and against a
+// teacher's top logits, with the error and the weight gradient, without the logits ever reaching memory.
+//
+// The reference ends in TiLinear.forward (ti_torch.py:241-253), TiLoss.forward (ti_loss.py:6-36) and TiLinear.backward (:255-266),
+// which write [rows][classes] logits and errors out and whose softmax has 11 bits: with 2048 equal classes every error is zero.
+// Here the softmax works on the int32 accumulators themselves:
+//
+//   a[t][v] = sum_f x[t][f] w[v][f],  e = exp_x + exp_w - temperature_log2
+//   E(d)    = 2^30 exp(-d 2^e) for whole d >= 0, in integers (exp_weight below; a quartic, |relative error| < 2.9e-6)
+//   pieces of 64 classes:  m_c = max a,  S_c = (sum E(m_c - a)) >> 6          (2^24 is 1)
+//   a row:  M = max m_c,  S = sum_c (S_c E(M - m_c)) >> 20                    (2^34 is 1)
+//   loss  = (M - a_y) 2^e + ln(S 2^-34)                                       (double, stored as float32)
+//   p     = hi32(E(M - a) R) >> (n - 3),  R = (2^63 - 1) / (S >> n), 2^31 <= S >> n < 2^32    (2^30 is 1; S >= 2^34, so n >= 3)
+//   err   = p - target share, narrowed by 23 bits to int8 (2^-7), NITI's roundings
+//
+// Sums of integers do not depend on their order, so tiles, splits and thread blocks change no bit of any result.
+//
+// Launches: vocab_stats_kernel (product + each piece's maximum and sum), vocab_entries_kernel (the logits of the wanted classes),
+// vocab_finish_kernel (row sums, loss, reciprocal, the errors of the wanted classes); for training, piece by piece of the
+// vocabulary, vocab_err_kernel (the product again, its errors as int8 in the workspace), vocab_patch_kernel and the two products
+// that lead back (umma_gemm), then the narrowing of the error.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <climits>
+#include <cstdint>
+
+#include "umma_core.cuh"
+#include "requant.cuh"
+
+namespace niti {
+namespace {
+
+constexpr int PIECE = 64;            // classes whose exponentials are summed relative to their own maximum: part of the definition
+constexpr int VBN = 256;             // columns of an output tile
+constexpr int VOCAB_EPI_WARPS = 16;  // four groups of four warps; a group owns 64 columns, a thread one row of them: one piece
+constexpr int VOCAB_THREADS = 64 + 32 * VOCAB_EPI_WARPS;
+constexpr int FINISH_THREADS = 256;
+constexpr int MAX_ENTRIES = 128;     // a teacher's logits per row
+
+// ---------------------------------------------------------------------------------------------- E(d)
+// u = d 2^e log2(e) in units of 2^-25, plus a half: its whole part I is the shift, its fraction less a half the polynomial's
+// argument in [-1/2, 1/2).  d 2^(26+e) has at most 31 bits once d is cut at D, where E is 0 (31 powers of two and more).
+struct ExpScale { unsigned D, K; int sl; };
+__device__ __forceinline__ ExpScale exp_scale(int e) {
+    ExpScale s;
+    if (e > 5) e = 5;  // from here on every d >= 1 gives 0
+    s.D = e >= 0 ? static_cast<unsigned>((21 + (1 << e)) >> e) : e <= -28 ? 0xFFFFFFFFu : 43u << (-e - 1);
+    s.sl = e >= -26 ? 26 + e : 0;
+    s.K = e >= -26 ? 0xB8AA3B29u : e <= -58 ? 0u : 0xB8AA3B29u >> (-26 - e);  // log2(e) 2^31
+    return s;
+}
+__device__ __forceinline__ uint32_t mad_hi(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("mad.hi.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ int32_t mad_hi(int32_t a, int32_t b, int32_t c) {
+    int32_t d;
+    asm("mad.hi.s32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t shift_right(uint32_t a, uint32_t n) {  // 0 for n >= 32, which the operator >> leaves undefined
+    uint32_t d;
+    asm("shr.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(n));
+    return d;
+}
+// xs = min(d, D) << sl
+__device__ __forceinline__ uint32_t exp_weight_shifted(uint32_t xs, uint32_t K) {
+    const uint32_t u = mad_hi(xs, K, 1u << 24);
+    const int32_t phi = static_cast<int32_t>((u << 7) + 0x80000000u);
+    int32_t q = mad_hi(phi, 10289510, -60029066);
+    q = mad_hi(phi, q, 257956795);
+    q = mad_hi(phi, q, -744236436);
+    q = mad_hi(phi, q, 1 << 30);
+    return shift_right(static_cast<uint32_t>(q), u >> 25);
+}
+__device__ __forceinline__ uint32_t exp_weight(uint32_t d, const ExpScale& s) { return exp_weight_shifted(min(d, s.D) << s.sl, s.K); }
+
+// A row's view of E: E(M - a) for its accumulators a <= M.  max(a, floor) cuts d at D; the difference is taken in the
+// multiply-add that shifts it (modulo 2^32, which the result stays below).
+struct RowExp { int32_t floor_a; uint32_t base; };
+__device__ __forceinline__ RowExp row_exp(int32_t M, const ExpScale& s) {
+    const long long f = static_cast<long long>(M) - s.D;
+    return {f < INT_MIN ? INT_MIN : static_cast<int32_t>(f), static_cast<uint32_t>(M) << s.sl};
+}
+__device__ __forceinline__ uint32_t exp_weight_row(int32_t a, const RowExp& r, uint32_t minus_unit, uint32_t K) {
+    return exp_weight_shifted(static_cast<uint32_t>(max(a, r.floor_a)) * minus_unit + r.base, K);
+}
+
+struct VocabParams {
+    GemmParams g;
+    const int32_t* exp_x; const int32_t* exp_w; int temperature;
+    int rows;                 // tokens
+    int first, classes;       // of the piece of the vocabulary this launch covers (multiple of 256); classes of the whole vocabulary
+    int32_t* piece_max; uint32_t* piece_sum;  // [pieces][rows]
+    const int4* row_stat;     // {M, R, n - 3, -}; R = 0: a row without an error
+    int8_t* err; long long err_pitch;
+    const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
+};
+
+template <bool TWO>
+struct VocabCfg {
+    static constexpr int B_STAGE_BYTES = (TWO ? VBN / 2 : VBN) * ROW_BYTES;
+    static constexpr int STAGE_BYTES = PANEL_BYTES + B_STAGE_BYTES;
+    static constexpr int STAGES = 224 * 1024 / STAGE_BYTES;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
+};
+
+// 64 columns of one row: the piece's maximum and its sum of exponentials.
+__device__ __forceinline__ void piece_stats(const uint32_t (&v)[64], int lim, const ExpScale& sc, uint32_t minus_unit, int32_t* m_out, uint32_t* s_out) {
+    int32_t m = INT_MIN;
+    unsigned long long sum = 0;
+    if (lim >= PIECE) {
+#pragma unroll
+        for (int i = 0; i < PIECE; i += 2) m = __vimax3_s32(m, static_cast<int>(v[i]), static_cast<int>(v[i + 1]));
+        const RowExp r = row_exp(m, sc);
+#pragma unroll
+        for (int i = 0; i < PIECE; i += 2)  // two of at most 2^30.5 fit in a word
+            sum += exp_weight_row(static_cast<int>(v[i]), r, minus_unit, sc.K) + exp_weight_row(static_cast<int>(v[i + 1]), r, minus_unit, sc.K);
+    } else {  // the vocabulary's last piece
+#pragma unroll
+        for (int i = 0; i < PIECE; ++i)
+            if (i < lim) m = max(m, static_cast<int>(v[i]));
+        const RowExp r = row_exp(m, sc);
+#pragma unroll
+        for (int i = 0; i < PIECE; ++i)
+            if (i < lim) sum += exp_weight_row(static_cast<int>(v[i]), r, minus_unit, sc.K);
+    }
+    *m_out = m;
+    *s_out = static_cast<uint32_t>(sum >> 6);
+}
+
+// p (2^30 is 1, never negative) -> int8 in units of 2^-7, packed four to a word.  The same values as narrow(p, 23, ...).
+template <int ROUND>
+__device__ __forceinline__ uint32_t narrow_p(uint32_t p, uint32_t rnd) {
+    if (ROUND == ROUND_NEAREST) return (p + (1u << 22)) >> 23;
+    const uint32_t lo = p & 0x7FFFFFu;
+    if (ROUND == ROUND_STOCHASTIC) return (p >> 23) + (lo > (rnd & 0x7FFFFFu) ? 1u : 0u);
+    return (p >> 23) + ((lo >> 11) > ((p << 1) & 0xFFEu) ? 1u : 0u);
+}
+
+enum { VOCAB_STATS = 3 };  // beside the three roundings of the error kernel
+
+// The product x w^T, tile by tile in tensor memory, and per row and 64 columns either the piece's statistics (WHAT == VOCAB_STATS) or
+// the errors as int8 in the workspace (WHAT: their rounding).  Roles, ring and accumulators are those of umma_gemm_kernel; sixteen
+// epilogue warps take a tile's 64-column groups out of tensor memory into registers, hand the accumulator back at once and work
+// on the registers under the next tile's MMAs.
+template <bool TWO, int WHAT>
+__global__ void __launch_bounds__(VOCAB_THREADS, 1)
+vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const VocabParams vp) {
+    using Cfg = VocabCfg<TWO>;
+    constexpr int STAGES = Cfg::STAGES;
+    const GemmParams& p = vp.g;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+    uint64_t* full_bar = bars;
+    uint64_t* empty_bar = bars + STAGES;
+    uint64_t* tfull_bar = bars + 2 * STAGES;
+    uint64_t* tempty_bar = bars + 2 * STAGES + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = TWO ? cluster_ctarank() : 0u;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(smem_u32(&full_bar[i]), 1); mbar_init(smem_u32(&empty_bar[i]), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&tfull_bar[i]), 1); mbar_init(smem_u32(&tempty_bar[i]), VOCAB_EPI_WARPS * (TWO ? 2 : 1)); }
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+    }
+    if (warp == 1) {
+        if (TWO) { tmem_alloc_pair(smem_u32(tmem_slot), 2 * VBN); tmem_relinquish_pair(); }
+        else     { tmem_alloc(smem_u32(tmem_slot), 2 * VBN); tmem_relinquish(); }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (TWO) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = p.m_tiles * p.n_tiles;
+    const int cta_first = TWO ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+    const int cta_step = TWO ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+
+    if (warp == 0) {
+        producer_role<VBN, STAGES, Cfg::STAGE_BYTES, TWO, false>(smem, full_bar, empty_bar, &tmA, &tmB, p, cta_first, cta_step, abort_flag);
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0)
+            mma_role<VBN, STAGES, Cfg::STAGE_BYTES, 2, TWO, false>(smem, full_bar, empty_bar, tfull_bar, tempty_bar, tmem_base, p, cta_first, cta_step, abort_flag);
+        __syncwarp();
+    } else {
+        const int grp = (warp - 2) >> 2, q = warp & 3;
+        const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+        const ExpScale sc = exp_scale(__ldg(vp.exp_x) + __ldg(vp.exp_w) - vp.temperature);
+        const uint32_t minus_unit = 0u - (1u << sc.sl);
+        unsigned long long seed = 0;
+        if (WHAT == ROUND_STOCHASTIC) seed = *vp.seed;
+        int it = 0;
+        for (int tile = cta_first; tile < total_tiles; tile += cta_step, ++it) {
+            const int acc = it & 1; const uint32_t aph = (it >> 1) & 1u;
+            int m_pair, n_t;
+            tile_coords(p, tile, &m_pair, &n_t);
+            const int m_t = TWO ? 2 * m_pair + static_cast<int>(rank) : m_pair;
+            const int row = m_t * BLOCK_M + q * 32 + lane;
+            const int col = n_t * VBN + grp * PIECE;  // within this launch's classes
+            const bool valid = row < vp.rows;
+            int4 stat = make_int4(0, 0, 0, 0);
+            if (WHAT != VOCAB_STATS && valid) stat = __ldg(vp.row_stat + row);
+            if (!mbar_wait_uniform(smem_u32(&tfull_bar[acc]), aph, abort_addr)) {
+                *abort_flag = 1;
+                if (lane == 0) report_abort(p.status, 4, 2);
+                break;
+            }
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * VBN + grp * PIECE);
+            uint32_t v[PIECE];
+            if (col < p.N) {
+                tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+                tmem_ld_32x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+                tmem_ld_wait();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (TWO) mbar_arrive_cluster(mapa_u32(smem_u32(&tempty_bar[acc]), 0));
+                else     mbar_arrive(smem_u32(&tempty_bar[acc]));
+            }
+            if (col >= p.N || !valid) continue;
+            if (WHAT == VOCAB_STATS) {
+                int32_t m; uint32_t s;
+                piece_stats(v, p.N - col, sc, minus_unit, &m, &s);
+                const long long at = static_cast<long long>(col / PIECE) * vp.rows + row;
+                vp.piece_max[at] = m;
+                vp.piece_sum[at] = s;
+            } else {
+                const RowExp r = row_exp(stat.x, sc);
+                const uint32_t R = static_cast<uint32_t>(stat.y), sh = static_cast<uint32_t>(stat.z);
+                int8_t* out = vp.err + row * vp.err_pitch + col;
+                const unsigned long long block0 =
+                    WHAT == ROUND_STOCHASTIC ? (vp.rng_offset + row) * static_cast<unsigned long long>((vp.classes + 3) >> 2) + ((vp.first + col) >> 2) : 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t rnd[4] = {0, 0, 0, 0}, y[4];
+                        if (WHAT == ROUND_STOCHASTIC) random_block(seed, vp.rng_stream, block0 + h * 8 + j, rnd);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t E = exp_weight_row(static_cast<int>(v[h * 32 + j * 4 + k]), r, minus_unit, sc.K);
+                            y[k] = narrow_p<WHAT>(__umulhi(E, R) >> sh, rnd[k]);
+                        }
+                        w[j] = __vminu4(y[0] | (y[1] << 8) | (y[2] << 16) | (y[3] << 24), 0x7F7F7F7Fu);
+                    }
+                    st_global_v8(out + h * 32, w);
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (TWO) cluster_sync_all();
+    if (warp == 1) {
+        if (*abort_flag) __nanosleep(200000);  // let copies and MMAs already in flight land
+        tc_fence_after();
+        __syncwarp();
+        if (TWO) tmem_dealloc_pair(tmem_base, 2 * VBN); else tmem_dealloc(tmem_base, 2 * VBN);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- wanted classes
+struct EntryParams {
+    const int8_t* x; const int8_t* w; int F16; int rows, classes, entries;
+    const long long* index;   // [rows][entries]: a class, or negative: none
+    int32_t* logit;           // [rows][entries]
+};
+// logit[t][k] = a[t][index[t][k]]: a warp to each, 512 bytes of both operands at a time
+__global__ void __launch_bounds__(256) vocab_entries_kernel(const EntryParams p) {
+    const long long i = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (i >= static_cast<long long>(p.rows) * p.entries) return;
+    const int lane = threadIdx.x & 31;
+    const long long j = p.index[i];
+    if (j < 0 || j >= p.classes) return;
+    const uint4* a = reinterpret_cast<const uint4*>(p.x) + (i / p.entries) * p.F16;
+    const uint4* b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
+    int sum = 0;
+    for (int c = lane; c < p.F16; c += 32) {
+        const uint4 u = __ldg(a + c), v = __ldg(b + c);
+        sum = __dp4a(static_cast<int>(u.x), static_cast<int>(v.x), sum);
+        sum = __dp4a(static_cast<int>(u.y), static_cast<int>(v.y), sum);
+        sum = __dp4a(static_cast<int>(u.z), static_cast<int>(v.z), sum);
+        sum = __dp4a(static_cast<int>(u.w), static_cast<int>(v.w), sum);
+    }
+    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+    if (lane == 0) p.logit[i] = sum;
+}
+
+struct FinishParams {
+    const int32_t* exp_x; const int32_t* exp_w; const int32_t* exp_top; int temperature;
+    int rows, classes, pieces, entries, rows_log2;  // a block's rows: 2^rows_log2
+    const int32_t* piece_max; const uint32_t* piece_sum;
+    const long long* index; long long ignore;  // ignore: the one negative class that is no mistake (a teacher's: every negative one)
+    const void* top; int top32;                // teacher's logits [rows][entries], int32 or int8; null: all on the one entry
+    const int32_t* logit;
+    float* loss;
+    int4* row_stat; int8_t* entry_err;         // null: the loss alone
+    int32_t* err_exp;
+    int round_mode;
+    const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
+};
+__device__ __forceinline__ double pow2(int e) { return scalbn(1.0, e); }
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+__global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const FinishParams p) {
+    __shared__ unsigned long long s_sum[FINISH_THREADS];
+    __shared__ int32_t s_max[FINISH_THREADS];
+    __shared__ unsigned s_share[FINISH_THREADS / 32][MAX_ENTRIES];
+    __shared__ int s_class[FINISH_THREADS / 32][MAX_ENTRIES];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int RB = 1 << p.rows_log2, G = FINISH_THREADS >> p.rows_log2;
+    const int r = tid & (RB - 1), g = tid >> p.rows_log2;
+    const int row0 = static_cast<int>(blockIdx.x) << p.rows_log2, row = row0 + r;
+    const int e = *p.exp_x + *p.exp_w - p.temperature;
+    const ExpScale sc = exp_scale(e);
+
+    // the row's maximum over its pieces, then its sum relative to it
+    int32_t m = INT_MIN;
+    if (row < p.rows) {
+#pragma unroll 4
+        for (int c = g; c < p.pieces; c += G) m = max(m, __ldg(p.piece_max + static_cast<long long>(c) * p.rows + row));
+    }
+    s_max[tid] = m;
+    __syncthreads();
+    for (int h = G >> 1; h > 0; h >>= 1) {
+        if (g < h) s_max[tid] = max(s_max[tid], s_max[tid + (h << p.rows_log2)]);
+        __syncthreads();
+    }
+    const int32_t M = s_max[r];
+    unsigned long long S = 0;
+    if (row < p.rows) {
+#pragma unroll 4
+        for (int c = g; c < p.pieces; c += G) {
+            const long long at = static_cast<long long>(c) * p.rows + row;
+            const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(__ldg(p.piece_max + at));
+            S += (static_cast<unsigned long long>(__ldg(p.piece_sum + at)) * exp_weight(d, sc)) >> 20;
+        }
+    }
+    s_sum[tid] = S;
+    __syncthreads();
+    for (int h = G >> 1; h > 0; h >>= 1) {
+        if (g < h) s_sum[tid] += s_sum[tid + (h << p.rows_log2)];
+        __syncthreads();
+    }
+
+    if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) *p.err_exp = p.temperature - 7;
+
+    // the wanted classes: a warp to each row, lane = entry
+    const double unit = pow2(max(-1000, min(1000, e)));
+    for (int i = warp; i < RB && row0 + i < p.rows; i += FINISH_THREADS / 32) {
+        const int t = row0 + i;
+        const unsigned long long Si = s_sum[i];
+        const int32_t Mi = s_max[i];
+        const int n = 32 - __clzll(static_cast<long long>(Si));
+        const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (Si >> n)), sh = static_cast<uint32_t>(n - 3);
+        const long long first = static_cast<long long>(t) * p.entries;
+        const ExpScale st = p.top != nullptr ? exp_scale(*p.exp_top - p.temperature) : ExpScale{0u, 0u, 0};
+        // which entries there are, and the teacher's largest
+        bool any = false, wrong = false;
+        int32_t best = INT_MIN;
+        for (int k = lane; k < p.entries; k += 32) {
+            const long long j = p.index[first + k];
+            const bool used = j >= 0 && j < p.classes;
+            wrong |= j >= p.classes || (p.top == nullptr && j < 0 && j != p.ignore);
+            any |= used;
+            s_class[warp][k] = used ? static_cast<int>(j) : -1;
+            if (used && p.top != nullptr)
+                best = max(best, p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]));
+        }
+        any = __any_sync(0xFFFFFFFFu, any);
+        wrong = __any_sync(0xFFFFFFFFu, wrong);
+        best = __reduce_max_sync(0xFFFFFFFFu, best);
+        unsigned long long total = 0;
+        for (int k = lane; k < p.entries; k += 32) {
+            unsigned share = 0;
+            if (s_class[warp][k] >= 0) {
+                share = 1u << 30;
+                if (p.top != nullptr) {
+                    const int32_t b = p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]);
+                    share = exp_weight(static_cast<unsigned>(best) - static_cast<unsigned>(b), st);
+                }
+            }
+            s_share[warp][k] = share;
+            total += share;
+        }
+        total = warp_sum(total);
+        const double ln_s = log(static_cast<double>(Si) * pow2(-34));
+        double loss = 0.0;
+        for (int k = lane; k < p.entries; k += 32) {
+            const unsigned share = s_share[warp][k];
+            if (s_class[warp][k] < 0) continue;
+            const double far = static_cast<double>(static_cast<long long>(Mi) - p.logit[first + k]) * unit + ln_s;  // -ln p
+            double own = 0.0;                                                                                       // ln q
+            if (p.top != nullptr) {
+                const int32_t b = p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]);
+                own = -static_cast<double>(static_cast<long long>(best) - b) * pow2(max(-1000, min(1000, *p.exp_top - p.temperature))) -
+                      log(static_cast<double>(total) * pow2(-30));
+            }
+            if (share != 0) loss += static_cast<double>(share) / static_cast<double>(total) * (far + own);
+            s_share[warp][k] = static_cast<unsigned>((static_cast<unsigned long long>(share) << 30) / total);
+        }
+        loss = warp_sum(loss) * pow2(2 * p.temperature);
+        const bool learns = any && !wrong;
+        if (lane == 0) p.loss[t] = wrong ? __int_as_float(0x7FC00000) : any ? static_cast<float>(loss) : 0.0f;
+        if (p.row_stat == nullptr) continue;
+        if (lane == 0) p.row_stat[t] = make_int4(Mi, learns ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), 0);
+        __syncwarp();
+        const unsigned long long seed = p.round_mode == ROUND_STOCHASTIC ? *p.seed : 0;
+        for (int k = lane; k < p.entries; k += 32) {
+            const int j = s_class[warp][k];
+            if (j < 0) continue;
+            int err = 0;
+            if (learns) {
+                unsigned q = 0;  // a class may be listed more than once
+                for (int o = 0; o < p.entries; ++o) q += s_class[warp][o] == j ? s_share[warp][o] : 0u;
+                const uint32_t E = exp_weight(static_cast<unsigned>(Mi) - static_cast<unsigned>(p.logit[first + k]), sc);
+                const int32_t v = static_cast<int32_t>(__umulhi(E, R) >> sh) - static_cast<int32_t>(q);
+                const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
+                err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
+            }
+            p.entry_err[first + k] = static_cast<int8_t>(err);
+        }
+        __syncwarp();
+    }
+}
+
+// the errors of the wanted classes of a piece of the vocabulary, over what vocab_kernel wrote there
+__global__ void __launch_bounds__(256) vocab_patch_kernel(const long long* index, const int8_t* entry_err, long long n, int entries, int first, int count,
+                                                          int8_t* err, long long pitch) {
+    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= n) return;
+    const long long j = index[i] - first;
+    if (index[i] >= 0 && j >= 0 && j < count) err[(i / entries) * pitch + j] = entry_err[i];
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+template <bool TWO, int WHAT>
+int launch_vocab_inst(const CUtensorMap& a, const CUtensorMap& b, const VocabParams& p, cudaStream_t st) {
+    using Cfg = VocabCfg<TWO>;
+    cudaError_t e = allow_shared<vocab_kernel<TWO, WHAT>>(Cfg::SMEM_BYTES);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    const int units = sm_count() / (TWO ? 2 : 1), tiles = p.g.m_tiles * p.g.n_tiles, grid = tiles < units ? tiles : units;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(VOCAB_THREADS); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = TWO ? 1 : 0;
+    return launched(cudaLaunchKernelEx(&cfg, vocab_kernel<TWO, WHAT>, a, b, p));
+}
+template <bool TWO>
+int launch_vocab(int what, const CUtensorMap& a, const CUtensorMap& b, const VocabParams& p, cudaStream_t st) {
+    switch (what) {
+        case ROUND_NEAREST: return launch_vocab_inst<TWO, ROUND_NEAREST>(a, b, p, st);
+        case ROUND_STOCHASTIC: return launch_vocab_inst<TWO, ROUND_STOCHASTIC>(a, b, p, st);
+        case ROUND_PSEUDO_STOCHASTIC: return launch_vocab_inst<TWO, ROUND_PSEUDO_STOCHASTIC>(a, b, p, st);
+        default: return launch_vocab_inst<TWO, VOCAB_STATS>(a, b, p, st);
+    }
+}
+// x [T][pitch] times `count` rows of w [V][pitch] from p->first on
+int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitch, int count, VocabParams* p, int32_t* status, cudaStream_t st) {
+    const int m128 = (T + 127) / 128;
+    const bool pair = (g_two_cta & 1) && m128 >= 2;
+    CUtensorMap ma, mb;
+    uint64_t dims[2] = {static_cast<uint64_t>(F), static_cast<uint64_t>(T)}, str[1] = {static_cast<uint64_t>(pitch)};
+    uint32_t box[2] = {128, 128};
+    if (int e = encode_map(&ma, x, false, 2, dims, str, box)) return e;
+    dims[1] = count; box[1] = pair ? VBN / 2 : VBN;
+    if (int e = encode_map(&mb, w + static_cast<long long>(p->first) * pitch, false, 2, dims, str, box)) return e;
+    GemmParams& g = p->g;
+    g = GemmParams{};
+    g.M = T; g.N = count; g.num_kb = (F + 127) / 128; g.splits = 1;
+    g.m_tiles = pair ? (m128 + 1) / 2 : m128; g.n_tiles = (count + VBN - 1) / VBN;
+    g.a_bytes = PANEL_BYTES; g.b_bytes = (pair ? VBN / 2 : VBN) * ROW_BYTES; g.mma_n = VBN;
+    g.status = status; g.nstages = g_stage_cap;
+    g.group_m = (static_cast<long long>(T) + count) * F > (48ll << 20) ? 8 : 0;  // as umma_gemm orders its tiles
+    g.fd_mn = make_fastdiv(g.m_tiles * g.n_tiles); g.fd_n = make_fastdiv(g.n_tiles); g.fd_tw = make_fastdiv(1); g.fd_th = make_fastdiv(1);
+    return pair ? launch_vocab<true>(what, ma, mb, *p, st) : launch_vocab<false>(what, ma, mb, *p, st);
+}
+
+size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+// The workspace of a call.
+struct VocabPlan {
+    int pieces, pitch, piece;   // row pitch of the operands; classes whose errors are in the workspace at a time
+    size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, g32_at, bytes;
+};
+constexpr long long ERR_BYTES = 64ll << 20;
+VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
+    VocabPlan p{};
+    p.pieces = (V + PIECE - 1) / PIECE;
+    p.pitch = (F + 15) / 16 * 16;
+    const int whole = (V + VBN - 1) / VBN * VBN;
+    long long piece = ERR_BYTES / T / VBN * VBN;
+    if (piece < VBN) piece = VBN;
+    p.piece = piece < whole ? static_cast<int>(piece) : whole;
+    size_t at = 0;
+    const auto take = [&](size_t n) { const size_t here = at; at = up(at + n, 256); return here; };
+    const size_t t = T, k = entries;
+    p.max_at = take(4 * t * p.pieces);
+    p.sum_at = take(4 * t * p.pieces);
+    p.logit_at = take(4 * t * k);
+    p.word_at = take(16);
+    if (p.pitch != F) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
+    if (train) {
+        p.stat_at = take(16 * t);
+        p.entry_at = take(t * k);
+        p.err_at = take(t * p.piece);
+        p.e32_at = take(4 * t * up(F, 4));
+        if (F % 4 != 0) p.g32_at = take(4 * up(F, 4) * (static_cast<size_t>(p.piece) > t ? p.piece : t));
+    }
+    p.bytes = at;
+    return p;
+}
+
+bool vocab_sizes_ok(long long T, long long F, long long V, long long entries) {
+    return T > 0 && F > 0 && V > 0 && entries > 0 && T < (1 << 17) && F < (1 << 17) && V <= (1 << 18) && entries <= MAX_ENTRIES;
+}
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+}  // namespace niti
+
+using namespace niti;
+
+extern "C" int niti_vocab_supported(int T, int F, int V, int entries) { return vocab_sizes_ok(T, F, V, entries) ? 1 : 0; }
+
+extern "C" size_t niti_vocab_scratch_bytes(int T, int F, int V, int entries, int train) {
+    return vocab_sizes_ok(T, F, V, entries) ? vocab_plan(T, F, V, entries, train != 0).bytes : 0;
+}
+
+extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
+    if (a == nullptr) return NITI_ERR_BAD_ARG;
+    const bool train = a->g32 != nullptr;
+    if (!(a->x && a->exp_x && a->w && a->exp_w && a->index && a->loss && a->scratch && a->T > 0 && a->F > 0 && a->V > 0 && a->entries > 0))
+        return NITI_ERR_BAD_ARG;
+    if ((a->top == nullptr) != (a->exp_top == nullptr) || (a->top == nullptr && a->entries != 1)) return NITI_ERR_BAD_ARG;
+    if (train && !(a->e8 && a->exp_err && a->grad_maxabs)) return NITI_ERR_BAD_ARG;
+    if (train && (!aligned16(a->e8) || !aligned16(a->g32))) return NITI_ERR_BAD_ARG;
+    if (train && (a->loss_round < 0 || a->loss_round > 2 || a->err_round < 0 || a->err_round > 2 ||
+                  (a->seed == nullptr && (a->loss_round == ROUND_STOCHASTIC || a->err_round == ROUND_STOCHASTIC))))
+        return NITI_ERR_BAD_ARG;
+    if (!vocab_sizes_ok(a->T, a->F, a->V, a->entries) || a->temperature_log2 < -30 || a->temperature_log2 > 30) return NITI_ERR_UNSUPPORTED;
+    const int T = a->T, F = a->F, V = a->V, K = a->entries;
+    const VocabPlan pl = vocab_plan(T, F, V, K, train);
+    if (!aligned16(a->scratch) || a->scratch_bytes < pl.bytes) return NITI_ERR_SCRATCH;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* ws = static_cast<char*>(a->scratch);
+
+    // operands whose rows are no multiples of 16 bytes go through copies that are
+    const int8_t *x = a->x, *w = a->w;
+    if (pl.pitch != F) {
+        x = reinterpret_cast<int8_t*>(ws + pl.x_at);
+        w = reinterpret_cast<int8_t*>(ws + pl.w_at);
+        // the bytes behind a row's end are read by vocab_entries_kernel only, against each other: zeros on one side will do
+        if (int e = set_cuda_error(cudaMemsetAsync(ws + pl.x_at, 0, static_cast<size_t>(T) * pl.pitch, st))) return e;
+        if (int e = copy_rows(a->x, F, ws + pl.x_at, pl.pitch, F, T, 1, st)) return e;
+        if (int e = copy_rows(a->w, F, ws + pl.w_at, pl.pitch, F, V, 1, st)) return e;
+    } else if (!aligned16(x) || !aligned16(w)) {
+        return NITI_ERR_BAD_ARG;
+    }
+
+    VocabParams vp{};
+    vp.exp_x = a->exp_x; vp.exp_w = a->exp_w; vp.temperature = a->temperature_log2;
+    vp.rows = T; vp.first = 0; vp.classes = V;
+    vp.piece_max = reinterpret_cast<int32_t*>(ws + pl.max_at); vp.piece_sum = reinterpret_cast<uint32_t*>(ws + pl.sum_at);
+    if (int e = run_vocab(VOCAB_STATS, x, w, T, F, pl.pitch, V, &vp, a->status, st)) return e;
+
+    EntryParams ep{x, w, pl.pitch / 16, T, V, K, reinterpret_cast<const long long*>(a->index), reinterpret_cast<int32_t*>(ws + pl.logit_at)};
+    const long long wanted = static_cast<long long>(T) * K;
+    vocab_entries_kernel<<<static_cast<unsigned>((wanted + 7) / 8), 256, 0, st>>>(ep);
+    if (int e = launched(cudaGetLastError())) return e;
+
+    FinishParams fp{};
+    fp.exp_x = a->exp_x; fp.exp_w = a->exp_w; fp.exp_top = a->exp_top; fp.temperature = a->temperature_log2;
+    fp.rows = T; fp.classes = V; fp.pieces = pl.pieces; fp.entries = K;
+    fp.rows_log2 = T >= 2048 ? 5 : T >= 256 ? 3 : 0;
+    fp.piece_max = vp.piece_max; fp.piece_sum = vp.piece_sum;
+    fp.index = ep.index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = ep.logit; fp.loss = a->loss;
+    int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|}
+    if (train) {
+        fp.row_stat = reinterpret_cast<int4*>(ws + pl.stat_at);
+        fp.entry_err = reinterpret_cast<int8_t*>(ws + pl.entry_at);
+        fp.err_exp = words;
+        fp.round_mode = a->loss_round;
+        fp.seed = reinterpret_cast<const unsigned long long*>(a->seed); fp.rng_stream = a->loss_stream; fp.rng_offset = a->sample_offset;
+    }
+    const int rb = 1 << fp.rows_log2;
+    vocab_finish_kernel<<<(T + rb - 1) / rb, FINISH_THREADS, 0, st>>>(fp);
+    if (int e = launched(cudaGetLastError())) return e;
+    if (!train) return NITI_OK;
+
+    vp.row_stat = fp.row_stat;
+    vp.err = reinterpret_cast<int8_t*>(ws + pl.err_at); vp.err_pitch = pl.piece;
+    vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
+    unsigned* e32_max = reinterpret_cast<unsigned*>(words + 1);
+    if (int e = clear_words(e32_max, 1, st)) return e;
+    if (int e = clear_words(a->grad_maxabs, 1, st)) return e;
+    const int F4 = static_cast<int>(up(F, 4));
+    int32_t* e32 = reinterpret_cast<int32_t*>(ws + pl.e32_at);
+    const bool one_piece = pl.piece >= V;
+    for (int v0 = 0; v0 < V; v0 += pl.piece) {
+        const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
+        vp.first = v0;
+        if (int e = run_vocab(a->loss_round, x, w, T, F, pl.pitch, count, &vp, a->status, st)) return e;
+        vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(fp.index, fp.entry_err, wanted, K, v0, count, vp.err, vp.err_pitch);
+        if (int e = launched(cudaGetLastError())) return e;
+        // e32 (+)= err w, g32 = err^T x
+        GemmExtra more{};
+        more.ldb = pl.pitch; more.accumulate = v0 > 0;
+        if (int e = umma_gemm(vp.err, w + static_cast<long long>(v0) * pl.pitch, e32, one_piece ? e32_max : nullptr, T, F, count, 0, 0, 1, nullptr, a->status, st,
+                              0, static_cast<int>(vp.err_pitch), F4, &more)) return e;
+        int32_t* g = a->g32 + static_cast<long long>(v0) * F;
+        int32_t* g_out = F % 4 == 0 ? g : reinterpret_cast<int32_t*>(ws + pl.g32_at);
+        more.accumulate = 0;
+        if (int e = umma_gemm(vp.err, x, g_out, a->grad_maxabs, count, F, T, 1, 0, 1, nullptr, a->status, st, 0, static_cast<int>(vp.err_pitch), F4, &more)) return e;
+        if (g_out != g) if (int e = copy_rows(g_out, 4ll * F4, g, 4ll * F, 4ll * F, count, 4, st)) return e;
+    }
+    int32_t* dense = e32;
+    if (F4 != F) {
+        dense = reinterpret_cast<int32_t*>(ws + pl.g32_at);
+        if (int e = copy_rows(e32, 4ll * F4, dense, 4ll * F, 4ll * F, T, 4, st)) return e;
+    }
+    if (!one_piece) if (int e = absmax_i32(dense, static_cast<long long>(T) * F, e32_max, st)) return e;
+    return niti_requant_i8(dense, a->e8, e32_max, static_cast<long long>(T) * F, NITI_CALC_ERR, a->bits, a->err_round, a->seed, a->err_stream,
+                           a->sample_offset * static_cast<uint64_t>(F), 0, words, a->exp_w, a->exp_err, nullptr, stream);
+}

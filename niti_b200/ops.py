@@ -409,6 +409,77 @@ def fc_head_train(x, exp_x, w, exp_w, target, seed, layer_stream, *, dropout=Tru
     return out8, exps[0], err8, e8, exps[1], g32, gm
 
 
+# ------------------------------------------------------------------ a vocabulary of classes
+def _vocab_work(x, w, index, train):
+    def work(r):
+        (T, F), V = x.shape, w.shape[0]
+        return (6 if train else 2) * T * V * F, T * F * (2 if train else 1) + V * F * (5 if train else 1) + 8 * index.numel() + 4 * T
+    return work
+
+
+def _vocab_no_tokens(x, exp_w, w, temperature_log2, g32):
+    """What a call without tokens returns: the same shapes, nothing to learn."""
+    g32 = torch.zeros(w.shape, dtype=torch.int32, device=w.device) if g32 is None else g32.zero_()
+    return (torch.empty(0, dtype=torch.float32, device=x.device), torch.empty_like(x), exp_w.reshape(()) + (temperature_log2 - 7), g32,
+            torch.zeros(1, dtype=torch.int32, device=x.device))
+
+
+def _vocab_call(layer, index, ignore_index, top, exp_top, temperature_log2, train):
+    x, exp_x, w, exp_w = layer
+    if x.dim() == 2 and x.shape[0] == 0:
+        _need_cuda(x, exp_x, w, exp_w, index)
+        r = _vocab_no_tokens(x, exp_w, w, temperature_log2, train[-1] if train else None)
+        return r if train else r[0]
+    # at most: operands in copies, statistics, wanted logits, row sums; words cleared, maximum, copy and narrowing of the error; per
+    # piece of errors the product again, the wanted errors, two products and a copy
+    launches = 5
+    if train:
+        launches += 5 + 5 * vocab_pieces(x.shape[0], w.shape[0])
+    return _run("niti_vocab_loss_i8", launches, _vocab_work(x, w, index, bool(train)), native.vocab_loss, x, exp_x, w, exp_w, index,
+                ignore_index, top, exp_top, temperature_log2, bool(train), *train)
+
+
+def vocab_pieces(tokens, classes):
+    """In how many pieces of the vocabulary a training call takes its errors (64 MB of them at a time)."""
+    piece = max(256, (64 << 20) // tokens // 256 * 256)
+    return (classes + piece - 1) // piece
+
+
+def vocab_loss(x, exp_x, w, exp_w, target, ignore_index=-100):
+    """Softmax cross entropy of a last layer with a vocabulary of classes, without its logits: x int8 [tokens, features] and
+    w int8 [classes, features] with their exponents, target int64 [tokens] -> float32 [tokens], -ln p of each token's class.
+    Rows whose target is ignore_index: 0.  Other targets outside the vocabulary: NaN."""
+    return _vocab_call((x, exp_x, w, exp_w), target, ignore_index, None, None, 0, ())
+
+
+def vocab_train(x, exp_x, w, exp_w, target, ignore_index=-100, *, bits=7, loss_mode=ROUND_PSEUDO_STOCHASTIC, err_mode=ROUND_NEAREST,
+                seed=None, loss_stream=0xFFFF, err_stream=1, sample_offset=0, g32=None):
+    """vocab_loss and the gradients of the sum of its losses: (loss float32 [tokens], e8 int8 [tokens, features], exp_err,
+    g32 int32 [classes, features], max|g32|).  (e8, exp_err) is the error of x; g32, the weight gradient in units of
+    2^(exp_x - 7), is what ops.update takes; a g32 that is given receives it.  loss_mode narrows the errors of the logits to int8
+    (units of 2^-7; rounding to nearest drops every probability below 2^-8, pseudo-stochastic below 2^-19), err_mode the error of
+    x.  Stochastic modes draw from the seed's streams loss_stream (round_up(classes, 4) words a token) and err_stream.  Rows
+    without a loss have no error."""
+    return _vocab_call((x, exp_x, w, exp_w), target, ignore_index, None, None, 0,
+                       (bits, loss_mode, err_mode, seed, loss_stream, err_stream, sample_offset, g32))
+
+
+def vocab_distill_loss(x, exp_x, w, exp_w, index, top, exp_top, temperature_log2=0):
+    """Distillation from a teacher's top logits: index int64 [tokens, entries] are the classes of its largest logits (any order;
+    negative: no entry), top (int8 or int32, same shape) with exp_top those logits.  float32 [tokens],
+    4^temperature_log2 * sum_k q_k (ln q_k - ln p[index_k]), q the softmax over the row's entries and p the student's over the
+    vocabulary, both at temperature 2^temperature_log2.  Rows without an entry: 0.  Rows with a class outside the vocabulary: NaN."""
+    return _vocab_call((x, exp_x, w, exp_w), index, -1, top, exp_top, temperature_log2, ())
+
+
+def vocab_distill_train(x, exp_x, w, exp_w, index, top, exp_top, temperature_log2=0, *, bits=7, loss_mode=ROUND_PSEUDO_STOCHASTIC,
+                        err_mode=ROUND_NEAREST, seed=None, loss_stream=0xFFFF, err_stream=1, sample_offset=0, g32=None):
+    """vocab_distill_loss and the gradients of the sum of its losses, as vocab_train returns them (g32 in units of
+    2^(exp_x - 7 + temperature_log2))."""
+    return _vocab_call((x, exp_x, w, exp_w), index, -1, top, exp_top, temperature_log2,
+                       (bits, loss_mode, err_mode, seed, loss_stream, err_stream, sample_offset, g32))
+
+
 def update(w, g32, maxabs, mu, mode=ROUND_PSEUDO_STOCHASTIC, seed=None, rng_stream=0):
     """In-place integer SGD update of the int8 weights from their int32 gradient accumulators."""
     def work(r):
