@@ -492,6 +492,11 @@ __device__ __forceinline__ void bulk_copy_cluster(uint32_t dst, uint32_t src, ui
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same arrival without release semantics, where what it hands over was only read (an accumulator copied to registers): a release
+// towards the cluster waits until the thread's earlier global stores, a tile's results, have been performed.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // TMA loads of a CTA pair: data lands in the executing CTA, the byte count is reported to `bar`, which
 // may live in either CTA of the pair (a shared::cluster address)
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y) {

@@ -32,7 +32,7 @@ namespace {
 
 constexpr int PIECE = 64;            // classes whose exponentials are summed relative to their own maximum: part of the definition
 constexpr int VBN = 256;             // columns of an output tile
-constexpr int VOCAB_EPI_WARPS = 16;  // four groups of four warps; a group owns 64 columns, a thread one row of them: one piece
+constexpr int VOCAB_EPI_WARPS = 16;  // four for each 64 columns of a tile; a thread works on one row of them: one piece
 constexpr int VOCAB_THREADS = 64 + 32 * VOCAB_EPI_WARPS;
 constexpr int FINISH_THREADS = 256;
 constexpr int MAX_ENTRIES = 128;     // a teacher's logits per row
@@ -49,15 +49,17 @@ __device__ __forceinline__ ExpScale exp_scale(int e) {
     s.K = e >= -26 ? 0xB8AA3B29u : e <= -58 ? 0u : 0xB8AA3B29u >> (-26 - e);  // log2(e) 2^31
     return s;
 }
-__device__ __forceinline__ uint32_t mad_hi(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("mad.hi.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
+// The high words of 32 x 32 bit products.  As the upper half of a 64-bit product with a separate addition: mad.hi, four cycles of the
+// multiplier as well, held back the instructions beside it (64 E's of a row: 37 cycles per 128 with mad.hi, 32 so).
+__device__ __forceinline__ uint32_t mul_hi(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mul.wide.u32 %0, %1, %2;" : "=l"(d) : "r"(a), "r"(b));
+    return static_cast<uint32_t>(d >> 32);
 }
-__device__ __forceinline__ int32_t mad_hi(int32_t a, int32_t b, int32_t c) {
-    int32_t d;
-    asm("mad.hi.s32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
+__device__ __forceinline__ int32_t mul_hi(int32_t a, int32_t b) {
+    int64_t d;
+    asm("mul.wide.s32 %0, %1, %2;" : "=l"(d) : "r"(a), "r"(b));
+    return static_cast<int32_t>(d >> 32);
 }
 __device__ __forceinline__ uint32_t shift_right(uint32_t a, uint32_t n) {  // 0 for n >= 32, which the operator >> leaves undefined
     uint32_t d;
@@ -66,13 +68,13 @@ __device__ __forceinline__ uint32_t shift_right(uint32_t a, uint32_t n) {  // 0 
 }
 // xs = min(d, D) << sl
 __device__ __forceinline__ uint32_t exp_weight_shifted(uint32_t xs, uint32_t K) {
-    const uint32_t u = mad_hi(xs, K, 1u << 24);
-    const int32_t phi = static_cast<int32_t>((u << 7) + 0x80000000u);
-    int32_t q = mad_hi(phi, 10289510, -60029066);
-    q = mad_hi(phi, q, 257956795);
-    q = mad_hi(phi, q, -744236436);
-    q = mad_hi(phi, q, 1 << 30);
-    return shift_right(static_cast<uint32_t>(q), u >> 25);
+    const uint32_t h = mul_hi(xs, K);
+    const int32_t phi = static_cast<int32_t>(h << 7);  // the fraction of h + 2^24, less a half, with 2^32 as 1
+    int32_t q = mul_hi(phi, 10289510) - 60029066;
+    q = mul_hi(phi, q) + 257956795;
+    q = mul_hi(phi, q) - 744236436;
+    q = mul_hi(phi, q) + (1 << 30);
+    return shift_right(static_cast<uint32_t>(q), (h + (1u << 24)) >> 25);
 }
 __device__ __forceinline__ uint32_t exp_weight(uint32_t d, const ExpScale& s) { return exp_weight_shifted(min(d, s.D) << s.sl, s.K); }
 
@@ -98,13 +100,132 @@ struct VocabParams {
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
 };
 
+// A stage of the ring holds 256 bytes of every row for a pair of thread blocks (two panels of A, two of the half of B) and 128 for a
+// single one.
 template <bool TWO>
 struct VocabCfg {
-    static constexpr int B_STAGE_BYTES = (TWO ? VBN / 2 : VBN) * ROW_BYTES;
-    static constexpr int STAGE_BYTES = PANEL_BYTES + B_STAGE_BYTES;
+    static constexpr int BLOCKS = TWO ? 2 : 1;  // 128-byte reduction blocks of a stage
+    static constexpr int B_PANEL_BYTES = (TWO ? VBN / 2 : VBN) * ROW_BYTES;
+    static constexpr int STAGE_BYTES = BLOCKS * (PANEL_BYTES + B_PANEL_BYTES);
     static constexpr int STAGES = 224 * 1024 / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
 };
+
+// ---------------------------------------------------------------------------------------------- loads and MMAs
+// The roles of umma_core.cuh for this one layout (both operands along the reduction), in half the instructions: the sixteen
+// epilogue warps keep the schedulers so busy that what the issuing warps execute per reduction block, not the tensor pipe, set
+// the pace (2048 features: 12400 cycles a tile with the general roles, 8900 where the epilogue computed nothing).
+template <bool TWO>
+__device__ __forceinline__ void vocab_load(uint8_t* smem, uint64_t* full_bar, uint64_t* empty_bar, const CUtensorMap* tmA, const CUtensorMap* tmB,
+                                           const GemmParams& p, int first, int step, volatile int* abort_flag) {
+    using Cfg = VocabCfg<TWO>;
+    const int total = keep_reg(p.m_tiles * p.n_tiles), num_kb = keep_reg(p.num_kb);
+    const uint32_t rank = TWO ? __shfl_sync(0xFFFFFFFFu, cluster_ctarank(), 0) : 0u;
+    const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+    const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar);
+    const uint32_t block_tx = static_cast<uint32_t>((TWO ? 2 : 1) * (PANEL_BYTES + Cfg::B_PANEL_BYTES));
+    uint32_t s = 0, ph = 1;
+    for (int tile = first; tile < total; tile += step) {
+        int m_pair, n_t;
+        tile_coords(p, tile, &m_pair, &n_t);
+        const int ya = (TWO ? 2 * m_pair + static_cast<int>(rank) : m_pair) * BLOCK_M;
+        const int yb = n_t * VBN + static_cast<int>(rank) * (VBN / 2);
+        for (int kb = 0; kb < num_kb; kb += Cfg::BLOCKS) {
+            mbar_wait_quiet(empty0 + 8 * s, ph, abort_addr);
+            const uint32_t sa = smem0 + s * Cfg::STAGE_BYTES;
+            if (elect_one()) {
+                const bool two = TWO && kb + 1 < num_kb;
+                uint32_t fb = full0 + 8 * s;
+                if (TWO) {
+                    if (rank == 0) mbar_arrive_expect_tx(fb, two ? 2 * block_tx : block_tx);
+                    fb = mapa_u32(fb, 0);
+                    tma_load_2d_pair(sa, tmA, fb, kb * ROW_BYTES, ya);
+                    tma_load_2d_pair(sa + 2 * PANEL_BYTES, tmB, fb, kb * ROW_BYTES, yb);
+                    if (two) {
+                        tma_load_2d_pair(sa + PANEL_BYTES, tmA, fb, (kb + 1) * ROW_BYTES, ya);
+                        tma_load_2d_pair(sa + 3 * PANEL_BYTES, tmB, fb, (kb + 1) * ROW_BYTES, yb);
+                    }
+                } else {
+                    mbar_arrive_expect_tx(fb, block_tx);
+                    tma_load_2d(sa, tmA, fb, kb * ROW_BYTES, ya);
+                    tma_load_2d(sa + PANEL_BYTES, tmB, fb, kb * ROW_BYTES, yb);
+                }
+            }
+            if (++s == Cfg::STAGES) { s = 0; ph ^= 1u; }
+        }
+    }
+    if (*abort_flag) report_abort(p.status, 1, 0);
+}
+
+// wait for a stage, MMAs of 32 reduction elements each (their descriptors differ in the low word), commit: one statement
+#define VOCAB_MMA(GROUP, AT, PRED)                                               \
+    "add.u32 x, %1, " AT ";\n\tmov.b64 a, {x, %3};\n\t"                         \
+    "add.u32 x, %2, " AT ";\n\tmov.b64 b, {x, %3};\n\t"                         \
+    "@E tcgen05.mma.cta_group::" GROUP ".kind::i8 [%0], a, b, %4, " PRED ";\n\t"
+template <bool TWO>
+__device__ __forceinline__ void vocab_mma_stage(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate,
+                                                uint32_t empty_bar, uint32_t full_bar, uint32_t parity, uint32_t abort_addr) {
+    if (TWO) {
+        asm volatile(
+            "{\n\t.reg .pred P, Q, E, T;\n\t.reg .b32 r, ab, x;\n\t.reg .u64 t0, t1;\n\t.reg .b64 a, b;\n\t"
+            NITI_QUIET_WAIT_ASM("VWP", "%7", "%8", "%9", "%10")
+            "elect.sync r|E, 0xFFFFFFFF;\n\tsetp.ne.b32 P, %5, 0;\n\tsetp.eq.b32 T, 0, 0;\n\t"
+            VOCAB_MMA("2", "0", "P") VOCAB_MMA("2", "2", "T") VOCAB_MMA("2", "4", "T") VOCAB_MMA("2", "6", "T")
+            VOCAB_MMA("2", "1024", "T") VOCAB_MMA("2", "1026", "T") VOCAB_MMA("2", "1028", "T") VOCAB_MMA("2", "1030", "T")
+            "@E tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%6], %11;\n\t}"
+            :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(empty_bar), "r"(full_bar), "r"(parity), "r"(abort_addr),
+               "l"(WAIT_LIMIT_NS), "h"(static_cast<uint16_t>(3))
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred P, Q, E, T;\n\t.reg .b32 r, ab, x;\n\t.reg .u64 t0, t1;\n\t.reg .b64 a, b;\n\t"
+            NITI_QUIET_WAIT_ASM("VW", "%7", "%8", "%9", "%10")
+            "elect.sync r|E, 0xFFFFFFFF;\n\tsetp.ne.b32 P, %5, 0;\n\tsetp.eq.b32 T, 0, 0;\n\t"
+            VOCAB_MMA("1", "0", "P") VOCAB_MMA("1", "2", "T") VOCAB_MMA("1", "4", "T") VOCAB_MMA("1", "6", "T")
+            "@E tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6];\n\t}"
+            :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(empty_bar), "r"(full_bar), "r"(parity), "r"(abort_addr),
+               "l"(WAIT_LIMIT_NS)
+            : "memory");
+    }
+}
+template <bool TWO>
+__device__ __forceinline__ void vocab_mma(uint8_t* smem, uint64_t* full_bar, uint64_t* empty_bar, uint64_t* tfull_bar, uint64_t* tempty_bar,
+                                          uint32_t tmem_base_in, const GemmParams& p, int first, int step, volatile int* abort_flag) {
+    using Cfg = VocabCfg<TWO>;
+    constexpr int STEPS = 4 * Cfg::BLOCKS;  // MMAs of a full stage
+    const int total = keep_reg(p.m_tiles * p.n_tiles), all_steps = keep_reg((p.K + 31) / 32);
+    const uint32_t idesc = make_idesc_i8(TWO ? 2 * BLOCK_M : BLOCK_M, VBN, 0, 0);
+    const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, tmem_base_in, 0);
+    const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
+    const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar);
+    const uint64_t a0 = make_smem_desc(smem_u32(smem), 16, 1024, SWIZZLE_128B_CODE);
+    const uint32_t lo0 = static_cast<uint32_t>(a0), hi = static_cast<uint32_t>(a0 >> 32);
+    uint32_t s = 0, ph = 0, it = 0;
+    for (int tile = first; tile < total; tile += step, ++it) {
+        const uint32_t acc = it & 1;
+        if (!mbar_wait_uniform(smem_u32(&tempty_bar[acc]), ((it >> 1) & 1u) ^ 1u, abort_addr)) { *abort_flag = 1; report_abort(p.status, 2, 1); break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * VBN;
+        for (int k = 0; k < all_steps; k += STEPS) {
+            const uint32_t a_lo = lo0 + s * (Cfg::STAGE_BYTES >> 4), b_lo = a_lo + ((Cfg::BLOCKS * PANEL_BYTES) >> 4);
+            if (all_steps - k >= STEPS) {
+                vocab_mma_stage<TWO>(d_tmem, a_lo, b_lo, hi, idesc, static_cast<uint32_t>(k), empty0 + 8 * s, full0 + 8 * s, ph, abort_addr);
+            } else {  // the reduction's end inside a stage
+                mbar_wait_quiet(full0 + 8 * s, ph, abort_addr);
+                if (elect_one()) {
+                    for (int j = 0; k + j < all_steps; ++j) {
+                        const uint32_t at = (j & 3) * 2 + (j >> 2) * (PANEL_BYTES >> 4);
+                        umma_issue<TWO>(d_tmem, (static_cast<uint64_t>(hi) << 32) | (a_lo + at), (static_cast<uint64_t>(hi) << 32) | (b_lo + at), idesc, static_cast<uint32_t>(k + j));
+                    }
+                    if (TWO) umma_commit_pair(empty0 + 8 * s); else umma_commit(empty0 + 8 * s);
+                }
+            }
+            if (++s == Cfg::STAGES) { s = 0; ph ^= 1u; }
+        }
+        if (elect_one()) { if (TWO) umma_commit_pair(smem_u32(&tfull_bar[acc])); else umma_commit(smem_u32(&tfull_bar[acc])); }
+    }
+    if (*abort_flag) report_abort(p.status, 3, 1);
+}
 
 // 64 columns of one row: the piece's maximum and its sum of exponentials.
 __device__ __forceinline__ void piece_stats(const uint32_t (&v)[64], int lim, const ExpScale& sc, uint32_t minus_unit, int32_t* m_out, uint32_t* s_out) {
@@ -130,13 +251,14 @@ __device__ __forceinline__ void piece_stats(const uint32_t (&v)[64], int lim, co
     *s_out = static_cast<uint32_t>(sum >> 6);
 }
 
-// p (2^30 is 1, never negative) -> int8 in units of 2^-7, packed four to a word.  The same values as narrow(p, 23, ...).
+// p (2^30 is 1, never negative) in units of 2^-7, 128 still to be cut to 127: the same values as narrow(p, 23, ...).  Pseudo-
+// stochastically p is rounded up where its twelve upper dropped bits A exceed twice the eleven lower ones, B: where A + 4095 - B
+// carries.
 template <int ROUND>
-__device__ __forceinline__ uint32_t narrow_p(uint32_t p, uint32_t rnd) {
-    if (ROUND == ROUND_NEAREST) return (p + (1u << 22)) >> 23;
-    const uint32_t lo = p & 0x7FFFFFu;
-    if (ROUND == ROUND_STOCHASTIC) return (p >> 23) + (lo > (rnd & 0x7FFFFFu) ? 1u : 0u);
-    return (p >> 23) + ((lo >> 11) > ((p << 1) & 0xFFEu) ? 1u : 0u);
+__device__ __forceinline__ int narrow_p(uint32_t p, uint32_t rnd) {
+    if (ROUND == ROUND_NEAREST) return static_cast<int>((p + (1u << 22)) >> 23);
+    if (ROUND == ROUND_STOCHASTIC) return static_cast<int>((p + (~rnd & 0x7FFFFFu)) >> 23);  // up where the dropped bits exceed the word's
+    return static_cast<int>((p + 0x7FF800u - ((p << 12) & 0x7FF000u)) >> 23);
 }
 
 enum { VOCAB_STATS = 3 };  // beside the three roundings of the error kernel
@@ -186,14 +308,14 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     const int cta_step = TWO ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
     if (warp == 0) {
-        producer_role<VBN, STAGES, Cfg::STAGE_BYTES, TWO, false>(smem, full_bar, empty_bar, &tmA, &tmB, p, cta_first, cta_step, abort_flag);
+        vocab_load<TWO>(smem, full_bar, empty_bar, &tmA, &tmB, p, cta_first, cta_step, abort_flag);
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0)
-            mma_role<VBN, STAGES, Cfg::STAGE_BYTES, 2, TWO, false>(smem, full_bar, empty_bar, tfull_bar, tempty_bar, tmem_base, p, cta_first, cta_step, abort_flag);
+            vocab_mma<TWO>(smem, full_bar, empty_bar, tfull_bar, tempty_bar, tmem_base, p, cta_first, cta_step, abort_flag);
         __syncwarp();
     } else {
-        const int grp = (warp - 2) >> 2, q = warp & 3;
+        const int piece = (warp - 2) >> 2, q = warp & 3;  // its 64 columns and 32 rows of every tile
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
         const ExpScale sc = exp_scale(__ldg(vp.exp_x) + __ldg(vp.exp_w) - vp.temperature);
         const uint32_t minus_unit = 0u - (1u << sc.sl);
@@ -206,7 +328,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             tile_coords(p, tile, &m_pair, &n_t);
             const int m_t = TWO ? 2 * m_pair + static_cast<int>(rank) : m_pair;
             const int row = m_t * BLOCK_M + q * 32 + lane;
-            const int col = n_t * VBN + grp * PIECE;  // within this launch's classes
+            const int col = n_t * VBN + piece * PIECE;  // within this launch's classes
             const bool valid = row < vp.rows;
             int4 stat = make_int4(0, 0, 0, 0);
             if (WHAT != VOCAB_STATS && valid) stat = __ldg(vp.row_stat + row);
@@ -216,7 +338,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 break;
             }
             tc_fence_after();
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * VBN + grp * PIECE);
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * VBN + piece * PIECE);
             uint32_t v[PIECE];
             if (col < p.N) {
                 tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
@@ -226,7 +348,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (TWO) mbar_arrive_cluster(mapa_u32(smem_u32(&tempty_bar[acc]), 0));
+                if (TWO) mbar_arrive_cluster_relaxed(mapa_u32(smem_u32(&tempty_bar[acc]), 0));
                 else     mbar_arrive(smem_u32(&tempty_bar[acc]));
             }
             if (col >= p.N || !valid) continue;
@@ -247,14 +369,15 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                     uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        uint32_t rnd[4] = {0, 0, 0, 0}, y[4];
+                        uint32_t rnd[4] = {0, 0, 0, 0};
+                        int y[4];
                         if (WHAT == ROUND_STOCHASTIC) random_block(seed, vp.rng_stream, block0 + h * 8 + j, rnd);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t E = exp_weight_row(static_cast<int>(v[h * 32 + j * 4 + k]), r, minus_unit, sc.K);
-                            y[k] = narrow_p<WHAT>(__umulhi(E, R) >> sh, rnd[k]);
+                            y[k] = narrow_p<WHAT>(mul_hi(E, R) >> sh, rnd[k]);
                         }
-                        w[j] = __vminu4(y[0] | (y[1] << 8) | (y[2] << 16) | (y[3] << 24), 0x7F7F7F7Fu);
+                        w[j] = pack2_sat_s8(y[1], y[0], pack2_sat_s8(y[3], y[2], 0u));
                     }
                     st_global_v8(out + h * 32, w);
                 }
@@ -437,7 +560,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
                 unsigned q = 0;  // a class may be listed more than once
                 for (int o = 0; o < p.entries; ++o) q += s_class[warp][o] == j ? s_share[warp][o] : 0u;
                 const uint32_t E = exp_weight(static_cast<unsigned>(Mi) - static_cast<unsigned>(p.logit[first + k]), sc);
-                const int32_t v = static_cast<int32_t>(__umulhi(E, R) >> sh) - static_cast<int32_t>(q);
+                const int32_t v = static_cast<int32_t>(mul_hi(E, R) >> sh) - static_cast<int32_t>(q);
                 const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
                 err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
             }
@@ -492,10 +615,9 @@ int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitc
     if (int e = encode_map(&mb, w + static_cast<long long>(p->first) * pitch, false, 2, dims, str, box)) return e;
     GemmParams& g = p->g;
     g = GemmParams{};
-    g.M = T; g.N = count; g.num_kb = (F + 127) / 128; g.splits = 1;
+    g.M = T; g.N = count; g.K = F; g.num_kb = (F + 127) / 128; g.splits = 1;
     g.m_tiles = pair ? (m128 + 1) / 2 : m128; g.n_tiles = (count + VBN - 1) / VBN;
-    g.a_bytes = PANEL_BYTES; g.b_bytes = (pair ? VBN / 2 : VBN) * ROW_BYTES; g.mma_n = VBN;
-    g.status = status; g.nstages = g_stage_cap;
+    g.status = status;
     g.group_m = (static_cast<long long>(T) + count) * F > (48ll << 20) ? 8 : 0;  // as umma_gemm orders its tiles
     g.fd_mn = make_fastdiv(g.m_tiles * g.n_tiles); g.fd_n = make_fastdiv(g.n_tiles); g.fd_tw = make_fastdiv(1); g.fd_th = make_fastdiv(1);
     return pair ? launch_vocab<true>(what, ma, mb, *p, st) : launch_vocab<false>(what, ma, mb, *p, st);
