@@ -538,6 +538,8 @@ typedef struct niti_vocab_args {
 } niti_vocab_args;
 NITI_API int niti_vocab_supported(int T, int F, int V, int entries);
 NITI_API size_t niti_vocab_scratch_bytes(int T, int F, int V, int entries, int train);
+/* classes whose errors a training call holds in scratch at a time (at most T times as many bytes) */
+NITI_API int niti_vocab_piece(int T, int V);
 NITI_API int niti_vocab_loss_i8(const niti_vocab_args* args, void* stream);
 
 /* TiFloatToInt8 + the NCHW -> NHWC permute of TiNet.forward (ti_torch.py:341-356, ti_net.py:18-19):

@@ -78,6 +78,7 @@ SIGNATURES = {
     "niti_fc_head_train_i8": (_i, [_p, _p]),
     "niti_vocab_supported": (_i, [_i] * 4),
     "niti_vocab_scratch_bytes": (_sz, [_i] * 5),
+    "niti_vocab_piece": (_i, [_i, _i]),
     "niti_vocab_loss_i8": (_i, [_p, _p]),
     "niti_dp_exchange_bytes": (_sz, []),
     "niti_peer_copy": (_i, [_p, _p, _sz, _p]),

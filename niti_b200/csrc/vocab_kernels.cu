@@ -89,13 +89,16 @@ __device__ __forceinline__ uint32_t exp_weight_row(int32_t a, const RowExp& r, u
     return exp_weight_shifted(static_cast<uint32_t>(max(a, r.floor_a)) * minus_unit + r.base, K);
 }
 
+// A row's wanted class and its error in a word, where a row has one: bits 0 to 17, bit 23 and bits 24 to 31.
+__device__ __forceinline__ int one_entry(int cls, int err) { return cls | (1 << 23) | (err << 24); }
+
 struct VocabParams {
     GemmParams g;
     const int32_t* exp_x; const int32_t* exp_w; int temperature;
     int rows;                 // tokens
     int first, classes;       // of the piece of the vocabulary this launch covers (multiple of 256); classes of the whole vocabulary
     int32_t* piece_max; uint32_t* piece_sum;  // [pieces][rows]
-    const int4* row_stat;     // {M, R, n - 3, -}; R = 0: a row without an error
+    const int4* row_stat;     // {M, R, n - 3, the wanted class where there is one: see one_entry}; R = 0: a row without an error
     int8_t* err; long long err_pitch;
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
 };
@@ -381,6 +384,8 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                     }
                     st_global_v8(out + h * 32, w);
                 }
+                const int at = (stat.w & 0x3FFFF) - vp.first - col;
+                if ((stat.w & (1 << 23)) && at >= 0 && at < PIECE) out[at] = static_cast<int8_t>(stat.w >> 24);
             }
         }
     }
@@ -402,25 +407,40 @@ struct EntryParams {
     const long long* index;   // [rows][entries]: a class, or negative: none
     int32_t* logit;           // [rows][entries]
 };
-// logit[t][k] = a[t][index[t][k]]: a warp to each, 512 bytes of both operands at a time
+__device__ __forceinline__ int dot16(const uint4& u, const uint4& v, int sum) {
+    sum = __dp4a(static_cast<int>(u.x), static_cast<int>(v.x), sum);
+    sum = __dp4a(static_cast<int>(u.y), static_cast<int>(v.y), sum);
+    sum = __dp4a(static_cast<int>(u.z), static_cast<int>(v.z), sum);
+    return __dp4a(static_cast<int>(u.w), static_cast<int>(v.w), sum);
+}
+// logit[t][k] = a[t][index[t][k]]: a warp to four entries of a row, 512 bytes of each operand at a time
+constexpr int ENTRIES_PER_WARP = 4;
 __global__ void __launch_bounds__(256) vocab_entries_kernel(const EntryParams p) {
+    const int groups = (p.entries + ENTRIES_PER_WARP - 1) / ENTRIES_PER_WARP;
     const long long i = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (i >= static_cast<long long>(p.rows) * p.entries) return;
-    const int lane = threadIdx.x & 31;
-    const long long j = p.index[i];
-    if (j < 0 || j >= p.classes) return;
-    const uint4* a = reinterpret_cast<const uint4*>(p.x) + (i / p.entries) * p.F16;
-    const uint4* b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
-    int sum = 0;
-    for (int c = lane; c < p.F16; c += 32) {
-        const uint4 u = __ldg(a + c), v = __ldg(b + c);
-        sum = __dp4a(static_cast<int>(u.x), static_cast<int>(v.x), sum);
-        sum = __dp4a(static_cast<int>(u.y), static_cast<int>(v.y), sum);
-        sum = __dp4a(static_cast<int>(u.z), static_cast<int>(v.z), sum);
-        sum = __dp4a(static_cast<int>(u.w), static_cast<int>(v.w), sum);
+    const long long row = i / groups;
+    if (row >= p.rows) return;
+    const int lane = threadIdx.x & 31, k0 = static_cast<int>(i - row * groups) * ENTRIES_PER_WARP;
+    const uint4* a = reinterpret_cast<const uint4*>(p.x) + row * p.F16;
+    const uint4* b[ENTRIES_PER_WARP];
+    int sum[ENTRIES_PER_WARP];
+#pragma unroll
+    for (int k = 0; k < ENTRIES_PER_WARP; ++k) {
+        const long long j = k0 + k < p.entries ? p.index[row * p.entries + k0 + k] : -1;
+        b[k] = reinterpret_cast<const uint4*>(p.w) + (j >= 0 && j < p.classes ? j : 0) * p.F16;  // any class where there is none: not looked at
+        sum[k] = 0;
     }
-    sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-    if (lane == 0) p.logit[i] = sum;
+#pragma unroll 2
+    for (int c = lane; c < p.F16; c += 32) {
+        const uint4 u = __ldg(a + c);
+#pragma unroll
+        for (int k = 0; k < ENTRIES_PER_WARP; ++k) sum[k] = dot16(u, __ldg(b[k] + c), sum[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < ENTRIES_PER_WARP; ++k) {
+        const int v = __reduce_add_sync(0xFFFFFFFFu, sum[k]);
+        if (lane == 0 && k0 + k < p.entries) p.logit[row * p.entries + k0 + k] = v;
+    }
 }
 
 struct FinishParams {
@@ -429,10 +449,12 @@ struct FinishParams {
     const int32_t* piece_max; const uint32_t* piece_sum;
     const long long* index; long long ignore;  // ignore: the one negative class that is no mistake (a teacher's: every negative one)
     const void* top; int top32;                // teacher's logits [rows][entries], int32 or int8; null: all on the one entry
-    const int32_t* logit;
+    int32_t* logit;                            // of the wanted classes; of a single one per row it is computed here
+    const int8_t* x; const int8_t* w; int F16;
     float* loss;
     int4* row_stat; int8_t* entry_err;         // null: the loss alone
-    int32_t* err_exp;
+    int32_t* err_exp; uint32_t* clear[2];      // training: written and zeroed for the launches behind
+    uint4* zero; long long zero_count;         // training: zeroed as well
     int round_mode;
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
 };
@@ -459,6 +481,20 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     const int row0 = static_cast<int>(blockIdx.x) << p.rows_log2, row = row0 + r;
     const int e = *p.exp_x + *p.exp_w - p.temperature;
     const ExpScale sc = exp_scale(e);
+
+    if (p.entries == 1 && warp < RB && row0 + warp < p.rows) {
+        const long long t = row0 + warp, j = p.index[t];
+        if (j >= 0 && j < p.classes) {
+            const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
+            int sum = 0;
+#pragma unroll 4
+            for (int c = lane; c < p.F16; c += 32) sum = dot16(__ldg(a + c), __ldg(b + c), sum);
+            sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+            if (lane == 0) p.logit[t] = sum;  // read by this lane alone
+        }
+    }
+    for (long long i = static_cast<long long>(blockIdx.x) * FINISH_THREADS + tid; i < p.zero_count; i += static_cast<long long>(gridDim.x) * FINISH_THREADS)
+        p.zero[i] = make_uint4(0, 0, 0, 0);
 
     // the row's maximum over its pieces, then its sum relative to it
     int32_t m = INT_MIN;
@@ -489,11 +525,11 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
         __syncthreads();
     }
 
-    if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) *p.err_exp = p.temperature - 7;
+    if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) { *p.err_exp = p.temperature - 7; *p.clear[0] = 0; *p.clear[1] = 0; }
 
     // the wanted classes: a warp to each row, lane = entry
     const double unit = pow2(max(-1000, min(1000, e)));
-    for (int i = warp; i < RB && row0 + i < p.rows; i += FINISH_THREADS / 32) {
+    for (int i = warp; i < RB && row0 + i < p.rows; i += FINISH_THREADS / 32) {  // RB <= 8: one
         const int t = row0 + i;
         const unsigned long long Si = s_sum[i];
         const int32_t Mi = s_max[i];
@@ -549,7 +585,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
         const bool learns = any && !wrong;
         if (lane == 0) p.loss[t] = wrong ? __int_as_float(0x7FC00000) : any ? static_cast<float>(loss) : 0.0f;
         if (p.row_stat == nullptr) continue;
-        if (lane == 0) p.row_stat[t] = make_int4(Mi, learns ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), 0);
+        int one = 0;
         __syncwarp();
         const unsigned long long seed = p.round_mode == ROUND_STOCHASTIC ? *p.seed : 0;
         for (int k = lane; k < p.entries; k += 32) {
@@ -564,8 +600,10 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
                 const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
                 err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
             }
-            p.entry_err[first + k] = static_cast<int8_t>(err);
+            if (p.entries == 1) one = one_entry(j, err);
+            else p.entry_err[first + k] = static_cast<int8_t>(err);
         }
+        if (lane == 0) p.row_stat[t] = make_int4(Mi, learns ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), one);
         __syncwarp();
     }
 }
@@ -630,15 +668,33 @@ struct VocabPlan {
     int pieces, pitch, piece;   // row pitch of the operands; classes whose errors are in the workspace at a time
     size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, g32_at, bytes;
 };
-constexpr long long ERR_BYTES = 64ll << 20;
+// Errors in the workspace at a time.  Pieces of 37 column tiles: 148 SMs are 74 pairs of thread blocks, so the errors' tiles and the weight
+// gradient's come in whole waves where the tokens, or the features, fill an even number of 256-row tiles.
+constexpr long long ERR_BYTES = 96ll << 20;
+constexpr int PIECE_TILES = 37;
+int vocab_piece(int T, int V) {
+    const long long whole = (V + VBN - 1) / VBN, most = ERR_BYTES / VBN / T;  // column tiles
+    const long long tiles = most >= whole ? whole : most >= PIECE_TILES ? most / PIECE_TILES * PIECE_TILES : most < 1 ? 1 : most;
+    return static_cast<int>(tiles) * VBN;
+}
+// In how many parts the reduction of the error's product is cut, which are added up: so that the last wave of tiles is not much
+// emptier than the others.  A tile costs its reduction blocks and about six more.
+int error_splits(int T, int F, int count) {
+    const int bn = F > 128 ? 256 : 128, m128 = (T + 127) / 128;
+    const bool pair = (g_two_cta & 1) && m128 >= 2 && bn == 256;
+    const int tiles = (pair ? (m128 + 1) / 2 : m128) * ((F + bn - 1) / bn), units = pair ? sm_count() / 2 : sm_count(), kb = (count + 127) / 128;
+    int best = 1, best_cost = INT_MAX;
+    for (int s = 1; s <= 32 && s * 4 <= kb + 3; ++s) {
+        const int cost = (tiles * s + units - 1) / units * ((kb + s - 1) / s + 6) + (s > 1 ? 4 : 0);
+        if (cost < best_cost) { best = s; best_cost = cost; }
+    }
+    return best;
+}
 VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     VocabPlan p{};
     p.pieces = (V + PIECE - 1) / PIECE;
     p.pitch = (F + 15) / 16 * 16;
-    const int whole = (V + VBN - 1) / VBN * VBN;
-    long long piece = ERR_BYTES / T / VBN * VBN;
-    if (piece < VBN) piece = VBN;
-    p.piece = piece < whole ? static_cast<int>(piece) : whole;
+    p.piece = vocab_piece(T, V);
     size_t at = 0;
     const auto take = [&](size_t n) { const size_t here = at; at = up(at + n, 256); return here; };
     const size_t t = T, k = entries;
@@ -673,6 +729,8 @@ extern "C" int niti_vocab_supported(int T, int F, int V, int entries) { return v
 extern "C" size_t niti_vocab_scratch_bytes(int T, int F, int V, int entries, int train) {
     return vocab_sizes_ok(T, F, V, entries) ? vocab_plan(T, F, V, entries, train != 0).bytes : 0;
 }
+
+extern "C" int niti_vocab_piece(int T, int V) { return T > 0 && V > 0 ? vocab_piece(T, V) : 0; }
 
 extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     if (a == nullptr) return NITI_ERR_BAD_ARG;
@@ -711,22 +769,31 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     vp.piece_max = reinterpret_cast<int32_t*>(ws + pl.max_at); vp.piece_sum = reinterpret_cast<uint32_t*>(ws + pl.sum_at);
     if (int e = run_vocab(VOCAB_STATS, x, w, T, F, pl.pitch, V, &vp, a->status, st)) return e;
 
-    EntryParams ep{x, w, pl.pitch / 16, T, V, K, reinterpret_cast<const long long*>(a->index), reinterpret_cast<int32_t*>(ws + pl.logit_at)};
+    const long long* index = reinterpret_cast<const long long*>(a->index);
+    int32_t* logit = reinterpret_cast<int32_t*>(ws + pl.logit_at);
     const long long wanted = static_cast<long long>(T) * K;
-    vocab_entries_kernel<<<static_cast<unsigned>((wanted + 7) / 8), 256, 0, st>>>(ep);
-    if (int e = launched(cudaGetLastError())) return e;
+    if (K > 1) {
+        const EntryParams ep{x, w, pl.pitch / 16, T, V, K, index, logit};
+        const long long warps = static_cast<long long>(T) * ((K + ENTRIES_PER_WARP - 1) / ENTRIES_PER_WARP);
+        vocab_entries_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, st>>>(ep);
+        if (int e = launched(cudaGetLastError())) return e;
+    }
 
     FinishParams fp{};
     fp.exp_x = a->exp_x; fp.exp_w = a->exp_w; fp.exp_top = a->exp_top; fp.temperature = a->temperature_log2;
     fp.rows = T; fp.classes = V; fp.pieces = pl.pieces; fp.entries = K;
-    fp.rows_log2 = T >= 2048 ? 5 : T >= 256 ? 3 : 0;
+    fp.rows_log2 = T >= 1024 ? 3 : T >= 256 ? 2 : 0;  // eight words of a piece fill a sector; few rows are better off in blocks of their own
     fp.piece_max = vp.piece_max; fp.piece_sum = vp.piece_sum;
-    fp.index = ep.index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = ep.logit; fp.loss = a->loss;
+    fp.index = index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = logit; fp.loss = a->loss;
+    fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16;
     int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|}
+    const int F4 = static_cast<int>(up(F, 4)), splits = train ? error_splits(T, F, pl.piece < V ? pl.piece : V) : 1;
+    const bool summed = train && (splits > 1 || pl.piece < V);  // e32 in several parts
     if (train) {
         fp.row_stat = reinterpret_cast<int4*>(ws + pl.stat_at);
         fp.entry_err = reinterpret_cast<int8_t*>(ws + pl.entry_at);
-        fp.err_exp = words;
+        fp.err_exp = words; fp.clear[0] = reinterpret_cast<uint32_t*>(words + 1); fp.clear[1] = a->grad_maxabs;
+        if (splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
         fp.round_mode = a->loss_round;
         fp.seed = reinterpret_cast<const unsigned long long*>(a->seed); fp.rng_stream = a->loss_stream; fp.rng_offset = a->sample_offset;
     }
@@ -739,21 +806,19 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     vp.err = reinterpret_cast<int8_t*>(ws + pl.err_at); vp.err_pitch = pl.piece;
     vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
     unsigned* e32_max = reinterpret_cast<unsigned*>(words + 1);
-    if (int e = clear_words(e32_max, 1, st)) return e;
-    if (int e = clear_words(a->grad_maxabs, 1, st)) return e;
-    const int F4 = static_cast<int>(up(F, 4));
     int32_t* e32 = reinterpret_cast<int32_t*>(ws + pl.e32_at);
-    const bool one_piece = pl.piece >= V;
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
         const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
         vp.first = v0;
         if (int e = run_vocab(a->loss_round, x, w, T, F, pl.pitch, count, &vp, a->status, st)) return e;
-        vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(fp.index, fp.entry_err, wanted, K, v0, count, vp.err, vp.err_pitch);
-        if (int e = launched(cudaGetLastError())) return e;
+        if (K > 1) {
+            vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(index, fp.entry_err, wanted, K, v0, count, vp.err, vp.err_pitch);
+            if (int e = launched(cudaGetLastError())) return e;
+        }
         // e32 (+)= err w, g32 = err^T x
         GemmExtra more{};
-        more.ldb = pl.pitch; more.accumulate = v0 > 0;
-        if (int e = umma_gemm(vp.err, w + static_cast<long long>(v0) * pl.pitch, e32, one_piece ? e32_max : nullptr, T, F, count, 0, 0, 1, nullptr, a->status, st,
+        more.ldb = pl.pitch; more.accumulate = v0 > 0 || splits > 1;
+        if (int e = umma_gemm(vp.err, w + static_cast<long long>(v0) * pl.pitch, e32, summed ? nullptr : e32_max, T, F, count, 0, 0, v0 == 0 ? splits : error_splits(T, F, count), nullptr, a->status, st,
                               0, static_cast<int>(vp.err_pitch), F4, &more)) return e;
         int32_t* g = a->g32 + static_cast<long long>(v0) * F;
         int32_t* g_out = F % 4 == 0 ? g : reinterpret_cast<int32_t*>(ws + pl.g32_at);
@@ -766,7 +831,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         dense = reinterpret_cast<int32_t*>(ws + pl.g32_at);
         if (int e = copy_rows(e32, 4ll * F4, dense, 4ll * F, 4ll * F, T, 4, st)) return e;
     }
-    if (!one_piece) if (int e = absmax_i32(dense, static_cast<long long>(T) * F, e32_max, st)) return e;
+    if (summed) if (int e = absmax_i32(dense, static_cast<long long>(T) * F, e32_max, st)) return e;
     return niti_requant_i8(dense, a->e8, e32_max, static_cast<long long>(T) * F, NITI_CALC_ERR, a->bits, a->err_round, a->seed, a->err_stream,
                            a->sample_offset * static_cast<uint64_t>(F), 0, words, a->exp_w, a->exp_err, nullptr, stream);
 }

@@ -440,8 +440,8 @@ def _vocab_call(layer, index, ignore_index, top, exp_top, temperature_log2, trai
 
 
 def vocab_pieces(tokens, classes):
-    """In how many pieces of the vocabulary a training call takes its errors (64 MB of them at a time)."""
-    piece = max(256, (64 << 20) // tokens // 256 * 256)
+    """In how many pieces of the vocabulary a training call takes its errors (up to 96 MB of them at a time)."""
+    piece = lib.niti_vocab_piece(tokens, classes)
     return (classes + piece - 1) // piece
 
 
