@@ -401,18 +401,183 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     }
 }
 
-// ---------------------------------------------------------------------------------------------- wanted classes
-struct EntryParams {
-    const int8_t* x; const int8_t* w; int F16; int rows, classes, entries;
-    const long long* index;   // [rows][entries]: a class, or negative: none
-    int32_t* logit;           // [rows][entries]
-};
+// ---------------------------------------------------------------------------------------------- operands of odd rows
+// Rows of `bytes` bytes, one behind the other from any address, to rows of a pitch of 16 bytes, the rest of each zeroed.  A thread to
+// 16 bytes: five aligned words and four funnel shifts; what lies across the tensor's ends is read byte by byte.
+__global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restrict__ src, uint4* __restrict__ dst, int bytes, int pitch16, long long pieces, long long total) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(src), end = begin + total;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += static_cast<long long>(gridDim.x) * 256) {
+        const long long row = i / pitch16;
+        const int c = static_cast<int>(i - row * pitch16) * 16, n = min(16, bytes - c);
+        const uintptr_t at = begin + row * bytes + c, word0 = at & ~uintptr_t(3);
+        uint32_t o[4];
+        if (word0 >= begin && word0 + 20 <= end) {
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(word0);
+            const uint32_t shift = static_cast<uint32_t>(at - word0) * 8;
+            uint32_t w[5];
+#pragma unroll
+            for (int k = 0; k < 5; ++k) w[k] = __ldg(p + k);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = __funnelshift_r(w[k], w[k + 1], shift);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                o[k] = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (4 * k + b < n) o[k] |= static_cast<uint32_t>(static_cast<uint8_t>(src[row * bytes + c + 4 * k + b])) << (8 * b);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // zeros behind the row's end
+            const int left = n - 4 * k;
+            if (left < 4) o[k] = left <= 0 ? 0u : o[k] & ((1u << (8 * left)) - 1u);
+        }
+        dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+int align_rows(const int8_t* src, void* dst, int bytes, int pitch, long long rows, cudaStream_t st) {
+    const long long pieces = rows * (pitch / 16), blocks = (pieces + 255) / 256, most = 16ll * sm_count();
+    vocab_align_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, st>>>(src, static_cast<uint4*>(dst), bytes, pitch / 16, pieces, rows * bytes);
+    return launched(cudaGetLastError());
+}
+
+// ---------------------------------------------------------------------------------------------- a few tokens
 __device__ __forceinline__ int dot16(const uint4& u, const uint4& v, int sum) {
     sum = __dp4a(static_cast<int>(u.x), static_cast<int>(v.x), sum);
     sum = __dp4a(static_cast<int>(u.y), static_cast<int>(v.y), sum);
     sum = __dp4a(static_cast<int>(u.z), static_cast<int>(v.z), sum);
     return __dp4a(static_cast<int>(u.w), static_cast<int>(v.w), sum);
 }
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// Up to THIN_TOKENS tokens: w passes once, at the rate of memory, and a 128-row tile of the tensor cores would hold next to nothing
+// (1 x 2048 x 131072: 48 us, 0.85 of the measured rate; as tiles 64).  A block takes pieces of 64 classes, a warp eight of them side by side; the features lie in
+// shared memory.  Rows of w that start off a 16-byte boundary are read from the boundary before, against a copy of the
+// features that starts as far behind one (zeros around it): no copy of w is needed.
+constexpr int THIN_TOKENS = 4, THIN_THREADS = 256, THIN_ROWS = PIECE / (THIN_THREADS / 32);
+constexpr size_t THIN_MAX_SMEM = 100 * 1024;  // two blocks to an SM (4 x 2047 x 65536, one block of 131 KB: 115 us; through the tensor cores 94)
+struct ThinParams {
+    const int8_t* x; long long x_pitch;       // [rows][x_pitch]
+    const int8_t* w; long long pitch;         // [classes][pitch], any address and pitch
+    int F, rows, classes, pieces, entries;
+    int step, copies, chunks;                 // rows of w start at (w + k step) mod 16; copies of the features; 16-byte chunks of a copy
+    const int32_t* exp_x; const int32_t* exp_w; int temperature;
+    int32_t* piece_max; uint32_t* piece_sum;
+    const long long* index; int32_t* logit;
+};
+template <int T, bool ALIGNED>
+__global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinParams p) {
+    extern __shared__ __align__(16) uint8_t thin_smem[];
+    __shared__ int32_t s_logit[T][PIECE];
+    uint4* sx = reinterpret_cast<uint4*>(thin_smem);  // [copies][T][chunks]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(p.w), end = begin + static_cast<uintptr_t>(p.classes - 1) * p.pitch + p.F;
+    const int base = static_cast<int>(begin & 15);
+    for (int i = tid; i < p.copies * T * p.chunks; i += THIN_THREADS) {
+        const int c = i % p.chunks, t = i / p.chunks % T, copy = i / p.chunks / T;
+        const int at = c * 16 - ((base + copy * p.step) & 15);  // the feature in the chunk's first byte
+        if (ALIGNED && c * 16 + 16 <= p.F && (reinterpret_cast<uintptr_t>(p.x) | static_cast<uintptr_t>(p.x_pitch)) % 16 == 0) {
+            sx[i] = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.x_pitch) + c);
+            continue;
+        }
+        uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < 16; ++b)
+            if (at + b >= 0 && at + b < p.F) o[b >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p.x[t * p.x_pitch + at + b])) << (8 * (b & 3));
+        sx[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    const ExpScale sc = exp_scale(*p.exp_x + *p.exp_w - p.temperature);
+    __syncthreads();
+    for (int piece = blockIdx.x; piece < p.pieces; piece += gridDim.x) {
+        const int row0 = piece * PIECE + warp * THIN_ROWS;
+        int sum[THIN_ROWS][T];
+        uintptr_t at[THIN_ROWS];
+        int copy[THIN_ROWS];
+        bool inside = true;  // no chunk of these rows crosses the tensor's ends
+#pragma unroll
+        for (int r = 0; r < THIN_ROWS; ++r) {
+            const uintptr_t start = begin + static_cast<uintptr_t>(min(row0 + r, p.classes - 1)) * p.pitch;  // rows behind the last: not looked at
+            at[r] = start & ~uintptr_t(15);
+            copy[r] = ALIGNED ? 0 : ((static_cast<int>(start & 15) - base) & 15) / p.step * T * p.chunks;
+            inside = inside && at[r] >= begin && at[r] + 16 * static_cast<uintptr_t>(p.chunks) <= end;
+#pragma unroll
+            for (int t = 0; t < T; ++t) sum[r][t] = 0;
+        }
+        if (inside) {
+#pragma unroll 1
+            for (int c = lane; c < p.chunks; c += 32) {
+                uint4 v[THIN_ROWS];
+#pragma unroll
+                for (int r = 0; r < THIN_ROWS; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(at[r]) + c);
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    uint4 u = sx[t * p.chunks + c];
+#pragma unroll
+                    for (int r = 0; r < THIN_ROWS; ++r) {
+                        if (!ALIGNED) u = sx[copy[r] + t * p.chunks + c];
+                        sum[r][t] = dot16(u, v[r], sum[r][t]);
+                    }
+                }
+            }
+        } else {
+            for (int c = lane; c < p.chunks; c += 32)
+#pragma unroll
+                for (int r = 0; r < THIN_ROWS; ++r) {
+                    uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int b = 0; b < 16; ++b) {
+                        const uintptr_t a = at[r] + 16 * c + b;
+                        if (a >= begin && a < end) o[b >> 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(a)) << (8 * (b & 3));
+                    }
+#pragma unroll
+                    for (int t = 0; t < T; ++t) sum[r][t] = dot16(sx[copy[r] + t * p.chunks + c], make_uint4(o[0], o[1], o[2], o[3]), sum[r][t]);
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < THIN_ROWS; ++r)
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const int v = __reduce_add_sync(0xFFFFFFFFu, sum[r][t]);
+                if (lane == 0) s_logit[t][warp * THIN_ROWS + r] = v;
+            }
+        __syncthreads();
+        if (warp < p.rows) {  // a warp to each token: the piece's statistics, and the wanted classes in it
+            const int lim = p.classes - piece * PIECE;
+            const int32_t a = lane < lim ? s_logit[warp][lane] : INT_MIN, b = lane + 32 < lim ? s_logit[warp][lane + 32] : INT_MIN;
+            const int32_t m = __reduce_max_sync(0xFFFFFFFFu, max(a, b));
+            unsigned long long e = 0;
+            if (lane < lim) e = exp_weight(static_cast<unsigned>(m) - static_cast<unsigned>(a), sc);
+            if (lane + 32 < lim) e += exp_weight(static_cast<unsigned>(m) - static_cast<unsigned>(b), sc);
+            e = warp_sum(e);
+            if (lane == 0) {
+                p.piece_max[static_cast<long long>(piece) * p.rows + warp] = m;
+                p.piece_sum[static_cast<long long>(piece) * p.rows + warp] = static_cast<uint32_t>(e >> 6);
+            }
+            for (int k = lane; k < p.entries; k += 32) {
+                const long long j = p.index[static_cast<long long>(warp) * p.entries + k] - static_cast<long long>(piece) * PIECE;
+                if (j >= 0 && j < PIECE && j < lim) p.logit[warp * p.entries + k] = s_logit[warp][j];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- wanted classes
+struct EntryParams {
+    const int8_t* x; const int8_t* w; int F16; int rows, classes, entries;
+    const long long* index;   // [rows][entries]: a class, or negative: none
+    int32_t* logit;           // [rows][entries]
+};
 // logit[t][k] = a[t][index[t][k]]: a warp to four entries of a row, 512 bytes of each operand at a time
 constexpr int ENTRIES_PER_WARP = 4;
 __global__ void __launch_bounds__(256) vocab_entries_kernel(const EntryParams p) {
@@ -450,7 +615,7 @@ struct FinishParams {
     const long long* index; long long ignore;  // ignore: the one negative class that is no mistake (a teacher's: every negative one)
     const void* top; int top32;                // teacher's logits [rows][entries], int32 or int8; null: all on the one entry
     int32_t* logit;                            // of the wanted classes; of a single one per row it is computed here
-    const int8_t* x; const int8_t* w; int F16;
+    const int8_t* x; const int8_t* w; int F16; // null: they are all there
     float* loss;
     int4* row_stat; int8_t* entry_err;         // null: the loss alone
     int32_t* err_exp; uint32_t* clear[2];      // training: written and zeroed for the launches behind
@@ -459,17 +624,6 @@ struct FinishParams {
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
 };
 __device__ __forceinline__ double pow2(int e) { return scalbn(1.0, e); }
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
-
 __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const FinishParams p) {
     __shared__ unsigned long long s_sum[FINISH_THREADS];
     __shared__ int32_t s_max[FINISH_THREADS];
@@ -482,7 +636,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     const int e = *p.exp_x + *p.exp_w - p.temperature;
     const ExpScale sc = exp_scale(e);
 
-    if (p.entries == 1 && warp < RB && row0 + warp < p.rows) {
+    if (p.x != nullptr && warp < RB && row0 + warp < p.rows) {
         const long long t = row0 + warp, j = p.index[t];
         if (j >= 0 && j < p.classes) {
             const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
@@ -663,6 +817,34 @@ int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitc
 
 size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+template <int T>
+int launch_thin_inst(const ThinParams& p, size_t smem, cudaStream_t st) {
+    const bool aligned = p.copies == 1;
+    cudaError_t e = aligned ? allow_shared<vocab_thin_kernel<T, true>>(THIN_MAX_SMEM) : allow_shared<vocab_thin_kernel<T, false>>(THIN_MAX_SMEM);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    // one piece to a block, dealt out by the hardware, unless the block has copies of the features to lay out first
+    const int most = sm_count() * (smem <= 48 * 1024 ? 4 : 2), grid = aligned || p.pieces < most ? p.pieces : most;
+    if (aligned) vocab_thin_kernel<T, true><<<grid, THIN_THREADS, smem, st>>>(p);
+    else         vocab_thin_kernel<T, false><<<grid, THIN_THREADS, smem, st>>>(p);
+    return launched(cudaGetLastError());
+}
+// How w's rows (of F bytes, `pitch` apart) lie to 16-byte boundaries, and the shared memory their features take.
+size_t thin_layout(int T, int F, long long pitch, const int8_t* w, ThinParams* p) {
+    p->step = 16;
+    for (int g = 8; g >= 1; g >>= 1) if (pitch % (2 * g) != 0) p->step = g;
+    p->copies = 16 / p->step;
+    p->chunks = (F + 15 + (p->copies == 1 && reinterpret_cast<uintptr_t>(w) % 16 == 0 ? 0 : 15)) / 16;
+    return static_cast<size_t>(p->copies) * T * p->chunks * 16;
+}
+int launch_thin(int T, const ThinParams& p, size_t smem, cudaStream_t st) {
+    switch (T) {
+        case 1: return launch_thin_inst<1>(p, smem, st);
+        case 2: return launch_thin_inst<2>(p, smem, st);
+        case 3: return launch_thin_inst<3>(p, smem, st);
+        default: return launch_thin_inst<4>(p, smem, st);
+    }
+}
+
 // The workspace of a call.
 struct VocabPlan {
     int pieces, pitch, piece;   // row pitch of the operands; classes whose errors are in the workspace at a time
@@ -690,6 +872,7 @@ int error_splits(int T, int F, int count) {
     }
     return best;
 }
+bool thin_serves(int T, int F) { ThinParams t{}; return T <= THIN_TOKENS && thin_layout(T, F, F, nullptr, &t) + 16 * 16 * T <= THIN_MAX_SMEM; }
 VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     VocabPlan p{};
     p.pieces = (V + PIECE - 1) / PIECE;
@@ -702,7 +885,7 @@ VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     p.sum_at = take(4 * t * p.pieces);
     p.logit_at = take(4 * t * k);
     p.word_at = take(16);
-    if (p.pitch != F) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
+    if (p.pitch != F && (train || !thin_serves(T, F))) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
     if (train) {
         p.stat_at = take(16 * t);
         p.entry_at = take(t * k);
@@ -752,14 +935,13 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
 
     // operands whose rows are no multiples of 16 bytes go through copies that are
     const int8_t *x = a->x, *w = a->w;
-    if (pl.pitch != F) {
+    const bool thin = thin_serves(T, F);
+    if (pl.pitch != F && (train || !thin)) {
         x = reinterpret_cast<int8_t*>(ws + pl.x_at);
         w = reinterpret_cast<int8_t*>(ws + pl.w_at);
-        // the bytes behind a row's end are read by vocab_entries_kernel only, against each other: zeros on one side will do
-        if (int e = set_cuda_error(cudaMemsetAsync(ws + pl.x_at, 0, static_cast<size_t>(T) * pl.pitch, st))) return e;
-        if (int e = copy_rows(a->x, F, ws + pl.x_at, pl.pitch, F, T, 1, st)) return e;
-        if (int e = copy_rows(a->w, F, ws + pl.w_at, pl.pitch, F, V, 1, st)) return e;
-    } else if (!aligned16(x) || !aligned16(w)) {
+        if (int e = align_rows(a->x, ws + pl.x_at, F, pl.pitch, T, st)) return e;
+        if (int e = align_rows(a->w, ws + pl.w_at, F, pl.pitch, V, st)) return e;
+    } else if (pl.pitch == F && (!aligned16(x) || !aligned16(w))) {
         return NITI_ERR_BAD_ARG;
     }
 
@@ -767,12 +949,21 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     vp.exp_x = a->exp_x; vp.exp_w = a->exp_w; vp.temperature = a->temperature_log2;
     vp.rows = T; vp.first = 0; vp.classes = V;
     vp.piece_max = reinterpret_cast<int32_t*>(ws + pl.max_at); vp.piece_sum = reinterpret_cast<uint32_t*>(ws + pl.sum_at);
-    if (int e = run_vocab(VOCAB_STATS, x, w, T, F, pl.pitch, V, &vp, a->status, st)) return e;
-
     const long long* index = reinterpret_cast<const long long*>(a->index);
     int32_t* logit = reinterpret_cast<int32_t*>(ws + pl.logit_at);
     const long long wanted = static_cast<long long>(T) * K;
-    if (K > 1) {
+    if (thin) {
+        ThinParams tp{};
+        tp.x = x; tp.w = w; tp.x_pitch = tp.pitch = w == a->w ? F : pl.pitch;
+        tp.F = F; tp.rows = T; tp.classes = V; tp.pieces = pl.pieces; tp.entries = K;
+        tp.exp_x = a->exp_x; tp.exp_w = a->exp_w; tp.temperature = a->temperature_log2;
+        tp.piece_max = vp.piece_max; tp.piece_sum = vp.piece_sum; tp.index = index; tp.logit = logit;
+        const size_t smem = thin_layout(T, F, tp.pitch, w, &tp);
+        if (int e = launch_thin(T, tp, smem, st)) return e;
+    } else if (int e = run_vocab(VOCAB_STATS, x, w, T, F, pl.pitch, V, &vp, a->status, st)) {
+        return e;
+    }
+    if (K > 1 && !thin) {
         const EntryParams ep{x, w, pl.pitch / 16, T, V, K, index, logit};
         const long long warps = static_cast<long long>(T) * ((K + ENTRIES_PER_WARP - 1) / ENTRIES_PER_WARP);
         vocab_entries_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, st>>>(ep);
@@ -785,7 +976,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     fp.rows_log2 = T >= 1024 ? 3 : T >= 256 ? 2 : 0;  // eight words of a piece fill a sector; few rows are better off in blocks of their own
     fp.piece_max = vp.piece_max; fp.piece_sum = vp.piece_sum;
     fp.index = index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = logit; fp.loss = a->loss;
-    fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16;
+    if (K == 1 && !thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
     int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|}
     const int F4 = static_cast<int>(up(F, 4)), splits = train ? error_splits(T, F, pl.piece < V ? pl.piece : V) : 1;
     const bool summed = train && (splits > 1 || pl.piece < V);  // e32 in several parts
