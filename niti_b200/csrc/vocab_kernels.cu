@@ -31,9 +31,9 @@ namespace niti {
 namespace {
 
 constexpr int PIECE = 64;            // classes whose exponentials are summed relative to their own maximum: part of the definition
-constexpr int VBN = 256;             // columns of an output tile
-constexpr int VOCAB_EPI_WARPS = 16;  // four for each 64 columns of a tile; a thread works on one row of them: one piece
-constexpr int VOCAB_THREADS = 64 + 32 * VOCAB_EPI_WARPS;
+constexpr int VBN = 256;             // columns of the widest output tile
+// Loading warp, MMA warp and four epilogue warps for each 64 columns of a tile; a thread works on one row of them: one piece.
+constexpr int vocab_threads(int bn) { return 64 + bn / PIECE * 128; }
 constexpr int FINISH_THREADS = 256;
 constexpr int MAX_ENTRIES = 128;     // a teacher's logits per row
 
@@ -105,10 +105,10 @@ struct VocabParams {
 
 // A stage of the ring holds 256 bytes of every row for a pair of thread blocks (two panels of A, two of the half of B) and 128 for a
 // single one.
-template <bool TWO>
+template <bool TWO, int BN>
 struct VocabCfg {
     static constexpr int BLOCKS = TWO ? 2 : 1;  // 128-byte reduction blocks of a stage
-    static constexpr int B_PANEL_BYTES = (TWO ? VBN / 2 : VBN) * ROW_BYTES;
+    static constexpr int B_PANEL_BYTES = (TWO ? BN / 2 : BN) * ROW_BYTES;
     static constexpr int STAGE_BYTES = BLOCKS * (PANEL_BYTES + B_PANEL_BYTES);
     static constexpr int STAGES = 224 * 1024 / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
@@ -118,10 +118,10 @@ struct VocabCfg {
 // The roles of umma_core.cuh for this one layout (both operands along the reduction), in half the instructions: the sixteen
 // epilogue warps keep the schedulers so busy that what the issuing warps execute per reduction block, not the tensor pipe, set
 // the pace (2048 features: 12400 cycles a tile with the general roles, 8900 where the epilogue computed nothing).
-template <bool TWO>
+template <bool TWO, int BN>
 __device__ __forceinline__ void vocab_load(uint8_t* smem, uint64_t* full_bar, uint64_t* empty_bar, const CUtensorMap* tmA, const CUtensorMap* tmB,
                                            const GemmParams& p, int first, int step, volatile int* abort_flag) {
-    using Cfg = VocabCfg<TWO>;
+    using Cfg = VocabCfg<TWO, BN>;
     const int total = keep_reg(p.m_tiles * p.n_tiles), num_kb = keep_reg(p.num_kb);
     const uint32_t rank = TWO ? __shfl_sync(0xFFFFFFFFu, cluster_ctarank(), 0) : 0u;
     const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
@@ -132,7 +132,7 @@ __device__ __forceinline__ void vocab_load(uint8_t* smem, uint64_t* full_bar, ui
         int m_pair, n_t;
         tile_coords(p, tile, &m_pair, &n_t);
         const int ya = (TWO ? 2 * m_pair + static_cast<int>(rank) : m_pair) * BLOCK_M;
-        const int yb = n_t * VBN + static_cast<int>(rank) * (VBN / 2);
+        const int yb = n_t * BN + static_cast<int>(rank) * (BN / 2);
         for (int kb = 0; kb < num_kb; kb += Cfg::BLOCKS) {
             mbar_wait_quiet(empty0 + 8 * s, ph, abort_addr);
             const uint32_t sa = smem0 + s * Cfg::STAGE_BYTES;
@@ -191,13 +191,13 @@ __device__ __forceinline__ void vocab_mma_stage(uint32_t d_tmem, uint32_t a_lo, 
             : "memory");
     }
 }
-template <bool TWO>
+template <bool TWO, int BN>
 __device__ __forceinline__ void vocab_mma(uint8_t* smem, uint64_t* full_bar, uint64_t* empty_bar, uint64_t* tfull_bar, uint64_t* tempty_bar,
                                           uint32_t tmem_base_in, const GemmParams& p, int first, int step, volatile int* abort_flag) {
-    using Cfg = VocabCfg<TWO>;
+    using Cfg = VocabCfg<TWO, BN>;
     constexpr int STEPS = 4 * Cfg::BLOCKS;  // MMAs of a full stage
     const int total = keep_reg(p.m_tiles * p.n_tiles), all_steps = keep_reg((p.K + 31) / 32);
-    const uint32_t idesc = make_idesc_i8(TWO ? 2 * BLOCK_M : BLOCK_M, VBN, 0, 0);
+    const uint32_t idesc = make_idesc_i8(TWO ? 2 * BLOCK_M : BLOCK_M, BN, 0, 0);
     const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, tmem_base_in, 0);
     const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
     const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar);
@@ -208,7 +208,7 @@ __device__ __forceinline__ void vocab_mma(uint8_t* smem, uint64_t* full_bar, uin
         const uint32_t acc = it & 1;
         if (!mbar_wait_uniform(smem_u32(&tempty_bar[acc]), ((it >> 1) & 1u) ^ 1u, abort_addr)) { *abort_flag = 1; report_abort(p.status, 2, 1); break; }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * VBN;
+        const uint32_t d_tmem = tmem_base + acc * BN;
         for (int k = 0; k < all_steps; k += STEPS) {
             const uint32_t a_lo = lo0 + s * (Cfg::STAGE_BYTES >> 4), b_lo = a_lo + ((Cfg::BLOCKS * PANEL_BYTES) >> 4);
             if (all_steps - k >= STEPS) {
@@ -267,13 +267,13 @@ __device__ __forceinline__ int narrow_p(uint32_t p, uint32_t rnd) {
 enum { VOCAB_STATS = 3 };  // beside the three roundings of the error kernel
 
 // The product x w^T, tile by tile in tensor memory, and per row and 64 columns either the piece's statistics (WHAT == VOCAB_STATS) or
-// the errors as int8 in the workspace (WHAT: their rounding).  Roles, ring and accumulators are those of umma_gemm_kernel; sixteen
-// epilogue warps take a tile's 64-column groups out of tensor memory into registers, hand the accumulator back at once and work
-// on the registers under the next tile's MMAs.
-template <bool TWO, int WHAT>
-__global__ void __launch_bounds__(VOCAB_THREADS, 1)
+// the errors as int8 in the workspace (WHAT: their rounding).  Roles, ring and accumulators are those of umma_gemm_kernel; the
+// epilogue warps (sixteen for 256 columns) take a tile's 64-column groups out of tensor memory into registers, hand the accumulator
+// back at once and work on the registers under the next tile's MMAs.
+template <bool TWO, int WHAT, int BN>
+__global__ void __launch_bounds__(vocab_threads(BN), 1)
 vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const VocabParams vp) {
-    using Cfg = VocabCfg<TWO>;
+    using Cfg = VocabCfg<TWO, BN>;
     constexpr int STAGES = Cfg::STAGES;
     const GemmParams& p = vp.g;
     extern __shared__ uint8_t smem_raw[];
@@ -291,15 +291,15 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) { mbar_init(smem_u32(&full_bar[i]), 1); mbar_init(smem_u32(&empty_bar[i]), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&tfull_bar[i]), 1); mbar_init(smem_u32(&tempty_bar[i]), VOCAB_EPI_WARPS * (TWO ? 2 : 1)); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&tfull_bar[i]), 1); mbar_init(smem_u32(&tempty_bar[i]), BN / PIECE * 4 * (TWO ? 2 : 1)); }
         *abort_flag = 0;
         fence_barrier_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
     }
     if (warp == 1) {
-        if (TWO) { tmem_alloc_pair(smem_u32(tmem_slot), 2 * VBN); tmem_relinquish_pair(); }
-        else     { tmem_alloc(smem_u32(tmem_slot), 2 * VBN); tmem_relinquish(); }
+        if (TWO) { tmem_alloc_pair(smem_u32(tmem_slot), 2 * BN); tmem_relinquish_pair(); }
+        else     { tmem_alloc(smem_u32(tmem_slot), 2 * BN); tmem_relinquish(); }
     }
     tc_fence_before();
     __syncthreads();
@@ -311,11 +311,11 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     const int cta_step = TWO ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
     if (warp == 0) {
-        vocab_load<TWO>(smem, full_bar, empty_bar, &tmA, &tmB, p, cta_first, cta_step, abort_flag);
+        vocab_load<TWO, BN>(smem, full_bar, empty_bar, &tmA, &tmB, p, cta_first, cta_step, abort_flag);
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0)
-            vocab_mma<TWO>(smem, full_bar, empty_bar, tfull_bar, tempty_bar, tmem_base, p, cta_first, cta_step, abort_flag);
+            vocab_mma<TWO, BN>(smem, full_bar, empty_bar, tfull_bar, tempty_bar, tmem_base, p, cta_first, cta_step, abort_flag);
         __syncwarp();
     } else {
         const int piece = (warp - 2) >> 2, q = warp & 3;  // its 64 columns and 32 rows of every tile
@@ -331,7 +331,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             tile_coords(p, tile, &m_pair, &n_t);
             const int m_t = TWO ? 2 * m_pair + static_cast<int>(rank) : m_pair;
             const int row = m_t * BLOCK_M + q * 32 + lane;
-            const int col = n_t * VBN + piece * PIECE;  // within this launch's classes
+            const int col = n_t * BN + piece * PIECE;  // within this launch's classes
             const bool valid = row < vp.rows;
             int4 stat = make_int4(0, 0, 0, 0);
             if (WHAT != VOCAB_STATS && valid) stat = __ldg(vp.row_stat + row);
@@ -341,7 +341,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 break;
             }
             tc_fence_after();
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * VBN + piece * PIECE);
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN + piece * PIECE);
             uint32_t v[PIECE];
             if (col < p.N) {
                 tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
@@ -397,7 +397,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         if (*abort_flag) __nanosleep(200000);  // let copies and MMAs already in flight land
         tc_fence_after();
         __syncwarp();
-        if (TWO) tmem_dealloc_pair(tmem_base, 2 * VBN); else tmem_dealloc(tmem_base, 2 * VBN);
+        if (TWO) tmem_dealloc_pair(tmem_base, 2 * BN); else tmem_dealloc(tmem_base, 2 * BN);
     }
 }
 
@@ -772,47 +772,51 @@ __global__ void __launch_bounds__(256) vocab_patch_kernel(const long long* index
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-template <bool TWO, int WHAT>
+template <bool TWO, int WHAT, int BN>
 int launch_vocab_inst(const CUtensorMap& a, const CUtensorMap& b, const VocabParams& p, cudaStream_t st) {
-    using Cfg = VocabCfg<TWO>;
-    cudaError_t e = allow_shared<vocab_kernel<TWO, WHAT>>(Cfg::SMEM_BYTES);
+    using Cfg = VocabCfg<TWO, BN>;
+    cudaError_t e = allow_shared<vocab_kernel<TWO, WHAT, BN>>(Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return set_cuda_error(e);
     const int units = sm_count() / (TWO ? 2 : 1), tiles = p.g.m_tiles * p.g.n_tiles, grid = tiles < units ? tiles : units;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(VOCAB_THREADS); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
+    cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(vocab_threads(BN)); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = TWO ? 1 : 0;
-    return launched(cudaLaunchKernelEx(&cfg, vocab_kernel<TWO, WHAT>, a, b, p));
+    return launched(cudaLaunchKernelEx(&cfg, vocab_kernel<TWO, WHAT, BN>, a, b, p));
 }
-template <bool TWO>
+template <bool TWO, int BN>
 int launch_vocab(int what, const CUtensorMap& a, const CUtensorMap& b, const VocabParams& p, cudaStream_t st) {
     switch (what) {
-        case ROUND_NEAREST: return launch_vocab_inst<TWO, ROUND_NEAREST>(a, b, p, st);
-        case ROUND_STOCHASTIC: return launch_vocab_inst<TWO, ROUND_STOCHASTIC>(a, b, p, st);
-        case ROUND_PSEUDO_STOCHASTIC: return launch_vocab_inst<TWO, ROUND_PSEUDO_STOCHASTIC>(a, b, p, st);
-        default: return launch_vocab_inst<TWO, VOCAB_STATS>(a, b, p, st);
+        case ROUND_NEAREST: return launch_vocab_inst<TWO, ROUND_NEAREST, BN>(a, b, p, st);
+        case ROUND_STOCHASTIC: return launch_vocab_inst<TWO, ROUND_STOCHASTIC, BN>(a, b, p, st);
+        case ROUND_PSEUDO_STOCHASTIC: return launch_vocab_inst<TWO, ROUND_PSEUDO_STOCHASTIC, BN>(a, b, p, st);
+        default: return launch_vocab_inst<TWO, VOCAB_STATS, BN>(a, b, p, st);
     }
 }
 // x [T][pitch] times `count` rows of w [V][pitch] from p->first on
 int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitch, int count, VocabParams* p, int32_t* status, cudaStream_t st) {
+    // A tile's 64-column groups share the SM's integer pipes: where all tiles of 64 or 128 columns find an SM of their own, a tile of 256
+    // takes longer (48 x 256 x 4096, 64 SMs instead of 16: the launch 11.8 -> 8.2 us).
     const int m128 = (T + 127) / 128;
-    const bool pair = (g_two_cta & 1) && m128 >= 2;
+    const int bn = m128 * ((count + 63) / 64) <= sm_count() ? 64 : m128 * ((count + 127) / 128) <= sm_count() ? 128 : VBN;
+    const bool pair = (g_two_cta & 1) && m128 >= 2 && bn == VBN;
     CUtensorMap ma, mb;
     uint64_t dims[2] = {static_cast<uint64_t>(F), static_cast<uint64_t>(T)}, str[1] = {static_cast<uint64_t>(pitch)};
     uint32_t box[2] = {128, 128};
     if (int e = encode_map(&ma, x, false, 2, dims, str, box)) return e;
-    dims[1] = count; box[1] = pair ? VBN / 2 : VBN;
+    dims[1] = count; box[1] = pair ? VBN / 2 : bn;
     if (int e = encode_map(&mb, w + static_cast<long long>(p->first) * pitch, false, 2, dims, str, box)) return e;
     GemmParams& g = p->g;
     g = GemmParams{};
     g.M = T; g.N = count; g.K = F; g.num_kb = (F + 127) / 128; g.splits = 1;
-    g.m_tiles = pair ? (m128 + 1) / 2 : m128; g.n_tiles = (count + VBN - 1) / VBN;
+    g.m_tiles = pair ? (m128 + 1) / 2 : m128; g.n_tiles = (count + bn - 1) / bn;
     g.status = status;
     g.group_m = (static_cast<long long>(T) + count) * F > (48ll << 20) ? 8 : 0;  // as umma_gemm orders its tiles
     g.fd_mn = make_fastdiv(g.m_tiles * g.n_tiles); g.fd_n = make_fastdiv(g.n_tiles); g.fd_tw = make_fastdiv(1); g.fd_th = make_fastdiv(1);
-    return pair ? launch_vocab<true>(what, ma, mb, *p, st) : launch_vocab<false>(what, ma, mb, *p, st);
+    if (pair) return launch_vocab<true, VBN>(what, ma, mb, *p, st);
+    return bn == 64 ? launch_vocab<false, 64>(what, ma, mb, *p, st) : bn == 128 ? launch_vocab<false, 128>(what, ma, mb, *p, st) : launch_vocab<false, VBN>(what, ma, mb, *p, st);
 }
 
 size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
