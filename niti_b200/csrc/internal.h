@@ -41,13 +41,21 @@ extern int g_stage_cap;  // experiments: cap on the shared-memory stages the GEM
 
 // tensor-core (tcgen05) paths, umma_kernels.cu; `out` is int32 (fused == null) or int8
 int umma_gemm_splits(int M, int N, int K);
-struct GemmExtra {
-    int ldb;         // row pitch of B in elements (0: dense)
-    int accumulate;  // 1: an int32 result is added to what is there (by TMA reductions), the splits of the reduction too; no maximum
-};
 int umma_gemm(const int8_t* A, const int8_t* B, void* out, unsigned* maxabs, int M, int N, int K, int trans_a,
               int trans_b, int splits, const FusedArgs* fused, int32_t* status, cudaStream_t st, int rows32 = 0,
-              int lda = 0, int ldc = 0, const GemmExtra* more = nullptr);  // row pitches of A and of an int32 result in elements (0: dense)
+              int lda = 0, int ldc = 0);  // row pitches of A and of an int32 result in elements (0: dense)
+// An int32 product: op(A) [M][K] op(B) [K][N], row pitches in elements (0: dense).  accumulate: the result, in `splits` parts of the
+// reduction, is added to what is there (by TMA reductions; no maximum then).
+struct GemmCall {
+    const int8_t* A; const int8_t* B; void* out; unsigned* maxabs;
+    int M, N, K, trans_a, trans_b, splits, lda, ldb, ldc, accumulate;
+    int32_t* status;
+};
+// Two products over the same number of columns in one launch, whose thread blocks are dealt out by work.  The plan cuts the first
+// one's reduction into `splits` parts: with more than one its call must accumulate, and no split may be empty (same sizes in both calls).
+struct GemmTwoPlan { int bn, splits, units, grid; bool pair; };
+GemmTwoPlan umma_gemm_two_plan(const GemmCall& first, const GemmCall& second);
+int umma_gemm_two(const GemmCall& first, const GemmCall& second, const GemmTwoPlan& plan, cudaStream_t st);
 int umma_conv(const int8_t* x, const int8_t* w, void* out, unsigned* maxabs, int Nimg, int H, int W, int C, int K,
               int R, int S, int pad, int flip, const FusedArgs* fused, int32_t* status, cudaStream_t st);
 // red / outc: reduction channels per tap, output channels; k3: 3x3 filters, padding 1

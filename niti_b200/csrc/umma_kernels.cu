@@ -19,6 +19,7 @@
 #include "umma_core.cuh"
 #include "requant.cuh"
 #include "grid_barrier.cuh"
+#include <climits>
 
 namespace niti {
 constexpr int GEMM_THREADS = 320;  // producer warp, MMA warp, two epilogue warpgroups of 4 warps
@@ -386,11 +387,10 @@ __device__ __forceinline__ void store_piece(int8_t* at, int cols, const uint32_t
     if (cols >= 32) *reinterpret_cast<uint4*>(at + 16) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// Plain products: int32 out (+ max|acc|).
+// Plain products: int32 out (+ max|acc|).  cta_first, cta_step: the tiles of this thread block (of a pair of them)
 template <int BN, bool TWO, bool ROWS32>
-__global__ void __launch_bounds__(GEMM_THREADS, 1)  // 10 warps: 3 on one scheduler -> at most 168 registers per thread
-umma_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmC, const GemmParams p) {
+__device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const GemmParams& p,
+                                          const int cta_first, const int cta_step) {
     using Cfg = GemmCfg<BN, TWO>;
     constexpr int STAGES = Cfg::STAGES;
 
@@ -431,8 +431,6 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
     const int mn_tiles = p.m_tiles * p.n_tiles;  // TWO: m_tiles counts 256-row tiles of the pair
     const int total_tiles = mn_tiles * p.splits;
-    const int cta_first = TWO ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
-    const int cta_step = TWO ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
     // Only one lane of warps 0 and 1 works; the others wait at __syncwarp so that each warp reaches the
     // block-wide barrier of the teardown converged (an aligned barrier executed by a diverged warp is undefined).
@@ -593,6 +591,22 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         __syncwarp();
         if (TWO) tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS); else tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
     }
+}
+template <int BN, bool TWO, bool ROWS32>
+__global__ void __launch_bounds__(GEMM_THREADS, 1)  // 10 warps: 3 on one scheduler -> at most 168 registers per thread
+umma_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmC, const GemmParams p) {
+    gemm_body<BN, TWO, ROWS32>(tmA, tmB, tmC, p, static_cast<int>(TWO ? blockIdx.x >> 1 : blockIdx.x), static_cast<int>(TWO ? gridDim.x >> 1 : gridDim.x));
+}
+// Two products in one launch, the first `units` thread blocks (pairs of them) at one and the others at the other.
+struct GemmTwoMaps { CUtensorMap a[2], b[2], c[2]; };
+struct GemmTwoParams { GemmParams job[2]; int units; };
+template <int BN, bool TWO>
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
+umma_gemm_two_kernel(const __grid_constant__ GemmTwoMaps maps, const __grid_constant__ GemmTwoParams tp) {
+    const int unit = static_cast<int>(TWO ? blockIdx.x >> 1 : blockIdx.x), all = static_cast<int>(TWO ? gridDim.x >> 1 : gridDim.x);
+    const int j = unit >= tp.units ? 1 : 0;
+    gemm_body<BN, TWO, false>(maps.a[j], maps.b[j], maps.c[j], tp.job[j], j ? unit - tp.units : unit, j ? all - tp.units : tp.units);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -2082,6 +2096,37 @@ int umma_gemm_splits(int M, int N, int K) {
     return splits < 1 ? 1 : splits;
 }
 
+// The tensor maps and parameters of a product.  out[splits][M][N] (splits == 1, or accumulate: the result itself)
+struct GemmMaps { CUtensorMap a, b, c; };
+static int gemm_setup(const GemmCall& g, int bn, bool pair, bool int32_out, GemmMaps* m, GemmParams* p) {
+    const int a_mn = g.trans_a ? 1 : 0, b_mn = g.trans_b ? 0 : 1;
+    uint64_t dims[2], str[1]; uint32_t box[2] = {128, 128};
+    if (a_mn) { dims[0] = g.M; dims[1] = g.K; str[0] = g.lda > 0 ? g.lda : g.M; } else { dims[0] = g.K; dims[1] = g.M; str[0] = g.lda > 0 ? g.lda : g.K; }
+    if (int e = encode_map(&m->a, g.A, false, 2, dims, str, box)) return e;
+    if (b_mn) { dims[0] = g.N; dims[1] = g.K; str[0] = g.ldb > 0 ? g.ldb : g.N; box[1] = 128; }
+    else      { dims[0] = g.K; dims[1] = g.N; str[0] = g.ldb > 0 ? g.ldb : g.K; box[1] = pair ? bn / 2 : bn; }
+    if (int e = encode_map(&m->b, g.B, false, 2, dims, str, box)) return e;
+    const uint64_t results = g.accumulate ? 1 : g.splits;
+    uint64_t dc[4] = {(uint64_t)g.N, (uint64_t)g.M, results, 1};
+    const uint64_t pitch = g.ldc > 0 ? g.ldc : g.N;
+    uint64_t sc[3] = {pitch * 4, g.M * pitch * 4, results * g.M * pitch * 4};
+    uint32_t bc[4] = {32, 128, 1, 1};
+    if (int32_out) if (int e = encode_map(&m->c, g.out, true, 4, dc, sc, bc)) return e;
+
+    p->conv = 0; p->M = g.M; p->N = g.N; p->num_kb = (g.K + 127) / 128; p->splits = g.splits;
+    p->m_tiles = (g.M + 127) / 128; p->n_tiles = (g.N + bn - 1) / bn;
+    if (pair) p->m_tiles = (p->m_tiles + 1) / 2;
+    p->a_mn = a_mn; p->b_mn = b_mn; p->a_bytes = PANEL_BYTES; p->b_bytes = (pair ? bn / 2 : bn) * ROW_BYTES;
+    p->mma_n = mma_columns(g.N, bn, p->n_tiles, pair);
+    p->K = g.K;
+    p->maxabs = g.splits > 1 || g.accumulate ? nullptr : g.maxabs; p->status = g.status;
+    p->accumulate = g.accumulate;
+    p->split_cols = (bn == 256 && p->m_tiles * p->n_tiles * g.splits <= 2 * (pair ? sm_count() / 2 : sm_count())) ? 1 : 0;
+    // operands beyond ~half of the 126 MB L2: order the tiles in compact groups
+    p->group_m = (static_cast<long long>(g.M) + g.N) * g.K > (48ll << 20) ? 8 : 0;
+    return 0;
+}
+
 // out[splits][M][N] (splits == 1: the result itself) = op(A) * op(B) over disjoint reduction ranges.
 // `fused` == null: int32 out; otherwise int8 out narrowed by the shift in fused->state[0] (splits must be 1).
 // rows32: operands of 32-byte rows as im2col32 writes them (1: A and B, K = 32; 2: B only, N = 32).  As boxes of a
@@ -2089,43 +2134,83 @@ int umma_gemm_splits(int M, int N, int K) {
 // a first layer (256 rows) took 4600 cycles, whatever its epilogue did.  3 -> 128 channels, 500 images: 109 -> 68 us
 // with the gather, 3 -> 64, 1024 images: the product alone 110 -> 44 us.
 int umma_gemm(const int8_t* A, const int8_t* B, void* out, unsigned* maxabs, int M, int N, int K, int trans_a,
-              int trans_b, int splits, const FusedArgs* fused, int32_t* status, cudaStream_t st, int rows32, int lda, int ldc,
-              const GemmExtra* more) {
-    CUtensorMap ma, mb, mc;
-    const int a_mn = trans_a ? 1 : 0, b_mn = trans_b ? 0 : 1;
+              int trans_b, int splits, const FusedArgs* fused, int32_t* status, cudaStream_t st, int rows32, int lda, int ldc) {
     const int bn = fused ? requant_bn(N, 1 << 20) : (N > 128) ? 256 : 128;
-    const bool pair = rows32 == 0 && !fused && pair_ok((M + 127) / 128, bn, b_mn, 0);
-    const bool accumulate = more && more->accumulate;
-    {
-        uint64_t dims[2], str[1]; uint32_t box[2] = {128, 128};
-        if (a_mn) { dims[0] = M; dims[1] = K; str[0] = lda > 0 ? lda : M; } else { dims[0] = K; dims[1] = M; str[0] = lda > 0 ? lda : K; }
-        if (int e = encode_map(&ma, A, false, 2, dims, str, box)) return e;
-        if (b_mn) { dims[0] = N; dims[1] = K; str[0] = N; box[1] = 128; } else { dims[0] = K; dims[1] = N; str[0] = K; box[1] = pair ? bn / 2 : bn; }
-        if (more && more->ldb > 0) str[0] = more->ldb;
-        if (int e = encode_map(&mb, B, false, 2, dims, str, box)) return e;
-        const uint64_t results = accumulate ? 1 : splits;
-        uint64_t dc[4] = {(uint64_t)N, (uint64_t)M, results, 1};
-        const uint64_t pitch = ldc > 0 ? ldc : N;
-        uint64_t sc[3] = {pitch * 4, M * pitch * 4, results * M * pitch * 4};
-        uint32_t bc[4] = {32, 128, 1, 1};
-        if (!fused) if (int e = encode_map(&mc, out, true, 4, dc, sc, bc)) return e;
-    }
+    const bool pair = rows32 == 0 && !fused && pair_ok((M + 127) / 128, bn, trans_b ? 0 : 1, 0);
+    GemmMaps m;
     GemmParams p{};
-    p.conv = 0; p.M = M; p.N = N; p.num_kb = (K + 127) / 128; p.splits = splits;
-    p.m_tiles = (M + 127) / 128; p.n_tiles = (N + bn - 1) / bn;
-    if (pair) p.m_tiles = (p.m_tiles + 1) / 2;
-    p.a_mn = a_mn; p.b_mn = b_mn; p.a_bytes = PANEL_BYTES; p.b_bytes = (pair ? bn / 2 : bn) * ROW_BYTES;
-    p.mma_n = rows32 == 2 ? 32 : mma_columns(N, bn, p.n_tiles, pair);
-    p.rows32 = rows32; p.a32 = A; p.b32 = B; p.K = K;
-    p.maxabs = splits > 1 || accumulate ? nullptr : maxabs; p.status = status;
-    p.accumulate = accumulate;
-    p.split_cols = (bn == 256 && p.m_tiles * p.n_tiles * splits <= 2 * (pair ? sm_count() / 2 : sm_count())) ? 1 : 0;
-    // operands beyond ~half of the 126 MB L2: order the tiles in compact groups
-    p.group_m = (static_cast<long long>(M) + N) * K > (48ll << 20) ? 8 : 0;
+    const GemmCall g{A, B, out, maxabs, M, N, K, trans_a, trans_b, splits, lda, 0, ldc, 0, status};
+    if (int e = gemm_setup(g, bn, pair, !fused, &m, &p)) return e;
+    if (rows32 == 2) p.mma_n = 32;
+    p.rows32 = rows32; p.a32 = A; p.b32 = B;
     set_fused(&p, fused);
     finish_params(&p);
-    if (fused) { p.out8 = static_cast<int8_t*>(out); return launch_requant(bn, false, rows32 ? LOAD_ROWS32 : LOAD_TAPS, false, fused->one, ma, mb, p, st); }
-    return launch_gemm(bn, pair, ma, mb, mc, p, st);
+    if (fused) { p.out8 = static_cast<int8_t*>(out); return launch_requant(bn, false, rows32 ? LOAD_ROWS32 : LOAD_TAPS, false, fused->one, m.a, m.b, p, st); }
+    return launch_gemm(bn, pair, m.a, m.b, m.c, p, st);
+}
+
+// A call's tiles and reduction blocks in a launch of `pair`s of thread blocks or single ones
+static void gemm_extent(const GemmCall& g, int bn, bool pair, int* tiles, int* kb) {
+    const int m = (g.M + 127) / 128;
+    *tiles = (pair ? (m + 1) / 2 : m) * ((g.N + bn - 1) / bn);
+    *kb = (g.K + 127) / 128;
+}
+GemmTwoPlan umma_gemm_two_plan(const GemmCall& first, const GemmCall& second) {
+    GemmTwoPlan best{};
+    best.bn = first.N > 128 || second.N > 128 ? 256 : 128;
+    best.pair = (g_two_cta & 1) && best.bn == 256 && first.M > BLOCK_M && second.M > BLOCK_M;
+    const int units = best.pair ? sm_count() / 2 : sm_count();
+    int t0, k0, t1, k1;
+    gemm_extent(first, best.bn, best.pair, &t0, &k0);
+    gemm_extent(second, best.bn, best.pair, &t1, &k1);
+    // waves of tiles times their reduction blocks and about six more (a tile's epilogue), the larger of the two
+    constexpr int PER_TILE = 6;
+    long long best_cost = LLONG_MAX;
+    const int cuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
+    for (const int s : cuts) {
+        if (s > 1 && 4 * s > k0) break;
+        const long long n0 = static_cast<long long>(t0) * s, c0 = (k0 + s - 1) / s + PER_TILE, c1 = k1 + PER_TILE;
+        const long long ideal = units * (n0 * c0) / (n0 * c0 + t1 * c1);
+        for (long long u = ideal - 1; u <= ideal + 2; ++u) {
+            long long u0 = u < 1 ? 1 : u > units - 1 ? units - 1 : u;
+            if (n0 + t1 <= units) u0 = n0;
+            const long long u1 = units - u0, a = (n0 + u0 - 1) / u0 * c0, b = (t1 + u1 - 1) / u1 * c1, cost = (a > b ? a : b) + (s > 1 ? 2 : 0);
+            if (cost < best_cost) { best_cost = cost; best.splits = s; best.units = static_cast<int>(u0 < n0 ? u0 : n0); best.grid = best.units + static_cast<int>(u1 < t1 ? u1 : t1); }
+        }
+    }
+    return best;
+}
+template <int BN, bool TWO>
+static int launch_gemm_two(const GemmTwoMaps& maps, const GemmTwoParams& tp, int grid, cudaStream_t st) {
+    using Cfg = GemmCfg<BN, TWO>;
+    cudaError_t e = allow_shared<umma_gemm_two_kernel<BN, TWO>>(Cfg::SMEM_BYTES);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(GEMM_THREADS); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = TWO ? 1 : 0;
+    return launched(cudaLaunchKernelEx(&cfg, umma_gemm_two_kernel<BN, TWO>, maps, tp));
+}
+int umma_gemm_two(const GemmCall& first, const GemmCall& second, const GemmTwoPlan& plan, cudaStream_t st) {
+    GemmTwoMaps maps;
+    GemmTwoParams tp{};
+    tp.units = plan.units;
+    for (int j = 0; j < 2; ++j) {
+        GemmCall g = j ? second : first;
+        if (!j) g.splits = plan.splits;
+        GemmMaps m;
+        if (int e = gemm_setup(g, plan.bn, plan.pair, true, &m, &tp.job[j])) return e;
+        maps.a[j] = m.a; maps.b[j] = m.b; maps.c[j] = m.c;
+        GemmParams& p = tp.job[j];
+        p.mma_n = mma_columns(g.N, plan.bn, p.n_tiles, plan.pair);
+        p.split_cols = plan.bn == 256 && p.m_tiles * p.n_tiles * p.splits <= 2 * (j ? plan.grid - plan.units : plan.units);
+        set_fused(&p, nullptr);
+        finish_params(&p);
+    }
+    return plan.bn == 256 ? (plan.pair ? launch_gemm_two<256, true>(maps, tp, plan.grid, st) : launch_gemm_two<256, false>(maps, tp, plan.grid, st))
+                          : launch_gemm_two<128, false>(maps, tp, plan.grid, st);
 }
 
 // Forward convolution (flip == 0: x [N,H,W,C] with w [K,R,S,C] -> [N,H,W,K]) or error-backward

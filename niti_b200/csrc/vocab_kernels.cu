@@ -863,19 +863,6 @@ int vocab_piece(int T, int V) {
     const long long tiles = most >= whole ? whole : most >= PIECE_TILES ? most / PIECE_TILES * PIECE_TILES : most < 1 ? 1 : most;
     return static_cast<int>(tiles) * VBN;
 }
-// In how many parts the reduction of the error's product is cut, which are added up: so that the last wave of tiles is not much
-// emptier than the others.  A tile costs its reduction blocks and about six more.
-int error_splits(int T, int F, int count) {
-    const int bn = F > 128 ? 256 : 128, m128 = (T + 127) / 128;
-    const bool pair = (g_two_cta & 1) && m128 >= 2 && bn == 256;
-    const int tiles = (pair ? (m128 + 1) / 2 : m128) * ((F + bn - 1) / bn), units = pair ? sm_count() / 2 : sm_count(), kb = (count + 127) / 128;
-    int best = 1, best_cost = INT_MAX;
-    for (int s = 1; s <= 32 && s * 4 <= kb + 3; ++s) {
-        const int cost = (tiles * s + units - 1) / units * ((kb + s - 1) / s + 6) + (s > 1 ? 4 : 0);
-        if (cost < best_cost) { best = s; best_cost = cost; }
-    }
-    return best;
-}
 bool thin_serves(int T, int F) { ThinParams t{}; return T <= THIN_TOKENS && thin_layout(T, F, F, nullptr, &t) + 16 * 16 * T <= THIN_MAX_SMEM; }
 VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     VocabPlan p{};
@@ -982,13 +969,28 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     fp.index = index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = logit; fp.loss = a->loss;
     if (K == 1 && !thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
     int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|}
-    const int F4 = static_cast<int>(up(F, 4)), splits = train ? error_splits(T, F, pl.piece < V ? pl.piece : V) : 1;
-    const bool summed = train && (splits > 1 || pl.piece < V);  // e32 in several parts
+    // e32 (+)= err w and g32 = err^T x of a piece of the vocabulary
+    const int F4 = static_cast<int>(up(F, 4));
+    int32_t* e32 = reinterpret_cast<int32_t*>(ws + pl.e32_at);
+    unsigned* e32_max = reinterpret_cast<unsigned*>(words + 1);
+    int8_t* err = reinterpret_cast<int8_t*>(ws + pl.err_at);
+    GemmCall to_x{}, to_w{};
+    const auto piece_calls = [&](int v0, int count) {
+        int32_t* g = F % 4 == 0 ? a->g32 + static_cast<long long>(v0) * F : reinterpret_cast<int32_t*>(ws + pl.g32_at);
+        to_x = GemmCall{err, w + static_cast<long long>(v0) * pl.pitch, e32, e32_max, T, F, count, 0, 0, 1, pl.piece, pl.pitch, F4, v0 > 0, a->status};
+        to_w = GemmCall{err, x, g, a->grad_maxabs, count, F, T, 1, 0, 1, pl.piece, pl.pitch, F4, 0, a->status};
+        const GemmTwoPlan plan = umma_gemm_two_plan(to_x, to_w);
+        if (plan.splits > 1) to_x.accumulate = 1;
+        return plan;
+    };
+    GemmTwoPlan plan{};
+    if (train) plan = piece_calls(0, pl.piece < V ? pl.piece : V);
+    const bool summed = train && (plan.splits > 1 || pl.piece < V);  // e32 comes in several parts
     if (train) {
         fp.row_stat = reinterpret_cast<int4*>(ws + pl.stat_at);
         fp.entry_err = reinterpret_cast<int8_t*>(ws + pl.entry_at);
         fp.err_exp = words; fp.clear[0] = reinterpret_cast<uint32_t*>(words + 1); fp.clear[1] = a->grad_maxabs;
-        if (splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
+        if (plan.splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
         fp.round_mode = a->loss_round;
         fp.seed = reinterpret_cast<const unsigned long long*>(a->seed); fp.rng_stream = a->loss_stream; fp.rng_offset = a->sample_offset;
     }
@@ -998,10 +1000,8 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     if (!train) return NITI_OK;
 
     vp.row_stat = fp.row_stat;
-    vp.err = reinterpret_cast<int8_t*>(ws + pl.err_at); vp.err_pitch = pl.piece;
+    vp.err = err; vp.err_pitch = pl.piece;
     vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
-    unsigned* e32_max = reinterpret_cast<unsigned*>(words + 1);
-    int32_t* e32 = reinterpret_cast<int32_t*>(ws + pl.e32_at);
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
         const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
         vp.first = v0;
@@ -1010,16 +1010,10 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
             vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(index, fp.entry_err, wanted, K, v0, count, vp.err, vp.err_pitch);
             if (int e = launched(cudaGetLastError())) return e;
         }
-        // e32 (+)= err w, g32 = err^T x
-        GemmExtra more{};
-        more.ldb = pl.pitch; more.accumulate = v0 > 0 || splits > 1;
-        if (int e = umma_gemm(vp.err, w + static_cast<long long>(v0) * pl.pitch, e32, summed ? nullptr : e32_max, T, F, count, 0, 0, v0 == 0 ? splits : error_splits(T, F, count), nullptr, a->status, st,
-                              0, static_cast<int>(vp.err_pitch), F4, &more)) return e;
-        int32_t* g = a->g32 + static_cast<long long>(v0) * F;
-        int32_t* g_out = F % 4 == 0 ? g : reinterpret_cast<int32_t*>(ws + pl.g32_at);
-        more.accumulate = 0;
-        if (int e = umma_gemm(vp.err, x, g_out, a->grad_maxabs, count, F, T, 1, 0, 1, nullptr, a->status, st, 0, static_cast<int>(vp.err_pitch), F4, &more)) return e;
-        if (g_out != g) if (int e = copy_rows(g_out, 4ll * F4, g, 4ll * F, 4ll * F, count, 4, st)) return e;
+        if (v0 > 0) plan = piece_calls(v0, count);
+        if (int e = umma_gemm_two(to_x, to_w, plan, st)) return e;
+        if (F % 4 != 0)
+            if (int e = copy_rows(to_w.out, 4ll * F4, a->g32 + static_cast<long long>(v0) * F, 4ll * F, 4ll * F, count, 4, st)) return e;
     }
     int32_t* dense = e32;
     if (F4 != F) {
