@@ -26,6 +26,7 @@
 
 #include "umma_core.cuh"
 #include "requant.cuh"
+#include "grid_barrier.cuh"
 
 namespace niti {
 namespace {
@@ -612,153 +613,194 @@ struct FinishParams {
     const int32_t* exp_x; const int32_t* exp_w; const int32_t* exp_top; int temperature;
     int rows, classes, pieces, entries, rows_log2;  // a block's rows: 2^rows_log2
     const int32_t* piece_max; const uint32_t* piece_sum;
-    const long long* index; long long ignore;  // ignore: the one negative class that is no mistake (a teacher's: every negative one)
+    const long long* index; long long ignore;  // ignore: rows of this class are left out (a teacher's: every negative one is)
     const void* top; int top32;                // teacher's logits [rows][entries], int32 or int8; null: all on the one entry
     int32_t* logit;                            // of the wanted classes; of a single one per row it is computed here
     const int8_t* x; const int8_t* w; int F16; // null: they are all there
     float* loss;
     int4* row_stat; int8_t* entry_err;         // null: the loss alone
-    int32_t* err_exp; uint32_t* clear[2];      // training: written and zeroed for the launches behind
+    int32_t* err_exp; uint32_t* clear[3];      // training: written and zeroed for the launches behind
     uint4* zero; long long zero_count;         // training: zeroed as well
     int round_mode;
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
 };
-__device__ __forceinline__ double pow2(int e) { return scalbn(1.0, e); }
+__device__ __forceinline__ double pow2(int e) { return __hiloint2double((1023 + max(-1022, min(1023, e))) << 20, 0); }
+// Row sums, losses, and for training what vocab_kernel needs of each row.  Up to eight rows to a block: a thread takes every G-th
+// piece of one of them, the first eight at once and into registers, so that a short vocabulary costs one trip to memory.
+// ONE: a class to each row, finished by a thread; otherwise a warp to each row, its lanes to the entries.
+constexpr int FINISH_HELD = 8;
+template <bool ONE>
 __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const FinishParams p) {
-    __shared__ unsigned long long s_sum[FINISH_THREADS];
-    __shared__ int32_t s_max[FINISH_THREADS];
-    __shared__ unsigned s_share[FINISH_THREADS / 32][MAX_ENTRIES];
-    __shared__ int s_class[FINISH_THREADS / 32][MAX_ENTRIES];
+    constexpr int WARPS = FINISH_THREADS / 32, MAX_ROWS = 8;
+    __shared__ unsigned long long s_sum[WARPS][MAX_ROWS];
+    __shared__ int32_t s_max[WARPS][MAX_ROWS], s_logit[MAX_ROWS];
+    __shared__ unsigned s_share[ONE ? 1 : WARPS][ONE ? 1 : MAX_ENTRIES];
+    __shared__ int s_class[ONE ? 1 : WARPS][ONE ? 1 : MAX_ENTRIES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int RB = 1 << p.rows_log2, G = FINISH_THREADS >> p.rows_log2;
     const int r = tid & (RB - 1), g = tid >> p.rows_log2;
     const int row0 = static_cast<int>(blockIdx.x) << p.rows_log2, row = row0 + r;
-    const int e = *p.exp_x + *p.exp_w - p.temperature;
-    const ExpScale sc = exp_scale(e);
+    const bool there = row < p.rows;
 
-    if (p.x != nullptr && warp < RB && row0 + warp < p.rows) {
-        const long long t = row0 + warp, j = p.index[t];
-        if (j >= 0 && j < p.classes) {
-            const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
-            int sum = 0;
-#pragma unroll 4
-            for (int c = lane; c < p.F16; c += 32) sum = dot16(__ldg(a + c), __ldg(b + c), sum);
-            sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-            if (lane == 0) p.logit[t] = sum;  // read by this lane alone
-        }
+    int32_t hm[FINISH_HELD];
+    uint32_t hs[FINISH_HELD];
+#pragma unroll
+    for (int u = 0; u < FINISH_HELD; ++u) {
+        const int c = g + u * G;
+        const bool in = there && c < p.pieces;
+        const long long at = static_cast<long long>(c) * p.rows + row;
+        hm[u] = in ? __ldg(p.piece_max + at) : INT_MIN;
+        hs[u] = in ? __ldg(p.piece_sum + at) : 0u;
     }
+    const int e = __ldg(p.exp_x) + __ldg(p.exp_w) - p.temperature;
+    const long long mine = ONE && tid < RB && there ? __ldg(p.index + row) : -1;
+    if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) { *p.err_exp = p.temperature - 7; *p.clear[0] = 0; *p.clear[1] = 0; *p.clear[2] = 0; }
     for (long long i = static_cast<long long>(blockIdx.x) * FINISH_THREADS + tid; i < p.zero_count; i += static_cast<long long>(gridDim.x) * FINISH_THREADS)
         p.zero[i] = make_uint4(0, 0, 0, 0);
+    if (ONE && warp < RB && row0 + warp < p.rows) {  // the wanted class's logit
+        const long long t = row0 + warp, j = __ldg(p.index + t);
+        if (j >= 0 && j < p.classes) {
+            int sum = 0;
+            if (p.x != nullptr) {
+                const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
+#pragma unroll 2
+                for (int c = lane; c < p.F16; c += 32) sum = dot16(__ldg(a + c), __ldg(b + c), sum);
+                sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+            } else {
+                sum = p.logit[t];
+            }
+            if (lane == 0) s_logit[warp] = sum;
+        }
+    }
 
     // the row's maximum over its pieces, then its sum relative to it
-    int32_t m = INT_MIN;
-    if (row < p.rows) {
-#pragma unroll 4
-        for (int c = g; c < p.pieces; c += G) m = max(m, __ldg(p.piece_max + static_cast<long long>(c) * p.rows + row));
+    int32_t m = hm[0];
+#pragma unroll
+    for (int u = 1; u < FINISH_HELD; ++u) m = max(m, hm[u]);
+    if (there) {
+#pragma unroll 8
+        for (int c = g + FINISH_HELD * G; c < p.pieces; c += G) m = max(m, __ldg(p.piece_max + static_cast<long long>(c) * p.rows + row));
     }
-    s_max[tid] = m;
+    for (int o = RB; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (lane < RB) s_max[warp][lane] = m;
     __syncthreads();
-    for (int h = G >> 1; h > 0; h >>= 1) {
-        if (g < h) s_max[tid] = max(s_max[tid], s_max[tid + (h << p.rows_log2)]);
-        __syncthreads();
-    }
-    const int32_t M = s_max[r];
+    m = s_max[0][r];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) m = max(m, s_max[w][r]);
+    const int32_t M = m;
+    const ExpScale sc = exp_scale(e);
     unsigned long long S = 0;
-    if (row < p.rows) {
+#pragma unroll 1
+    for (int u = 0; u < FINISH_HELD; ++u) {
+        // (a loop around one copy of E: this code runs once, and what a thread block has to fetch of it takes longer than it runs)
+        int32_t mu = hm[0]; uint32_t su = hs[0];
+#pragma unroll
+        for (int k = 1; k < FINISH_HELD; ++k) if (k == u) { mu = hm[k]; su = hs[k]; }
+        if (g + u * G >= p.pieces) break;
+        S += (static_cast<unsigned long long>(su) * exp_weight(static_cast<unsigned>(M) - static_cast<unsigned>(mu), sc)) >> 20;
+    }
+    if (there) {
 #pragma unroll 4
-        for (int c = g; c < p.pieces; c += G) {
+        for (int c = g + FINISH_HELD * G; c < p.pieces; c += G) {
             const long long at = static_cast<long long>(c) * p.rows + row;
             const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(__ldg(p.piece_max + at));
             S += (static_cast<unsigned long long>(__ldg(p.piece_sum + at)) * exp_weight(d, sc)) >> 20;
         }
     }
-    s_sum[tid] = S;
+    for (int o = RB; o < 32; o <<= 1) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
+    if (lane < RB) s_sum[warp][lane] = S;
     __syncthreads();
-    for (int h = G >> 1; h > 0; h >>= 1) {
-        if (g < h) s_sum[tid] += s_sum[tid + (h << p.rows_log2)];
-        __syncthreads();
-    }
 
-    if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) { *p.err_exp = p.temperature - 7; *p.clear[0] = 0; *p.clear[1] = 0; }
-
-    // the wanted classes: a warp to each row, lane = entry
-    const double unit = pow2(max(-1000, min(1000, e)));
-    for (int i = warp; i < RB && row0 + i < p.rows; i += FINISH_THREADS / 32) {  // RB <= 8: one
-        const int t = row0 + i;
-        const unsigned long long Si = s_sum[i];
-        const int32_t Mi = s_max[i];
-        const int n = 32 - __clzll(static_cast<long long>(Si));
-        const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (Si >> n)), sh = static_cast<uint32_t>(n - 3);
-        const long long first = static_cast<long long>(t) * p.entries;
-        const ExpScale st = p.top != nullptr ? exp_scale(*p.exp_top - p.temperature) : ExpScale{0u, 0u, 0};
-        // which entries there are, and the teacher's largest
-        bool any = false, wrong = false;
-        int32_t best = INT_MIN;
-        for (int k = lane; k < p.entries; k += 32) {
-            const long long j = p.index[first + k];
-            const bool used = j >= 0 && j < p.classes;
-            wrong |= j >= p.classes || (p.top == nullptr && j < 0 && j != p.ignore);
-            any |= used;
-            s_class[warp][k] = used ? static_cast<int>(j) : -1;
-            if (used && p.top != nullptr)
-                best = max(best, p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]));
-        }
-        any = __any_sync(0xFFFFFFFFu, any);
-        wrong = __any_sync(0xFFFFFFFFu, wrong);
-        best = __reduce_max_sync(0xFFFFFFFFu, best);
-        unsigned long long total = 0;
-        for (int k = lane; k < p.entries; k += 32) {
-            unsigned share = 0;
-            if (s_class[warp][k] >= 0) {
-                share = 1u << 30;
-                if (p.top != nullptr) {
-                    const int32_t b = p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]);
-                    share = exp_weight(static_cast<unsigned>(best) - static_cast<unsigned>(b), st);
-                }
-            }
-            s_share[warp][k] = share;
-            total += share;
-        }
-        total = warp_sum(total);
-        const double ln_s = log(static_cast<double>(Si) * pow2(-34));
-        double loss = 0.0;
-        for (int k = lane; k < p.entries; k += 32) {
-            const unsigned share = s_share[warp][k];
-            if (s_class[warp][k] < 0) continue;
-            const double far = static_cast<double>(static_cast<long long>(Mi) - p.logit[first + k]) * unit + ln_s;  // -ln p
-            double own = 0.0;                                                                                       // ln q
-            if (p.top != nullptr) {
-                const int32_t b = p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]);
-                own = -static_cast<double>(static_cast<long long>(best) - b) * pow2(max(-1000, min(1000, *p.exp_top - p.temperature))) -
-                      log(static_cast<double>(total) * pow2(-30));
-            }
-            if (share != 0) loss += static_cast<double>(share) / static_cast<double>(total) * (far + own);
-            s_share[warp][k] = static_cast<unsigned>((static_cast<unsigned long long>(share) << 30) / total);
-        }
-        loss = warp_sum(loss) * pow2(2 * p.temperature);
-        const bool learns = any && !wrong;
-        if (lane == 0) p.loss[t] = wrong ? __int_as_float(0x7FC00000) : any ? static_cast<float>(loss) : 0.0f;
-        if (p.row_stat == nullptr) continue;
+    const double unit = pow2(e);
+    if (ONE) {
+        if (tid >= RB || !there) return;
+        S = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) S += s_sum[w][tid];
+        const bool used = mine >= 0 && mine < p.classes && mine != p.ignore, wrong = !used && mine != p.ignore;
+        const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(s_logit[tid]);
+        float loss = wrong ? __int_as_float(0x7FC00000) : 0.0f;
+        if (used) loss = static_cast<float>(static_cast<double>(d) * unit + log(static_cast<double>(S) * pow2(-34)));
+        p.loss[row] = loss;
+        if (p.row_stat == nullptr) return;
+        const int n = 32 - __clzll(static_cast<long long>(S));
+        const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (S >> n)), sh = static_cast<uint32_t>(n - 3);
         int one = 0;
-        __syncwarp();
-        const unsigned long long seed = p.round_mode == ROUND_STOCHASTIC ? *p.seed : 0;
-        for (int k = lane; k < p.entries; k += 32) {
-            const int j = s_class[warp][k];
-            if (j < 0) continue;
-            int err = 0;
-            if (learns) {
-                unsigned q = 0;  // a class may be listed more than once
-                for (int o = 0; o < p.entries; ++o) q += s_class[warp][o] == j ? s_share[warp][o] : 0u;
-                const uint32_t E = exp_weight(static_cast<unsigned>(Mi) - static_cast<unsigned>(p.logit[first + k]), sc);
-                const int32_t v = static_cast<int32_t>(mul_hi(E, R) >> sh) - static_cast<int32_t>(q);
-                const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
-                err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
-            }
-            if (p.entries == 1) one = one_entry(j, err);
-            else p.entry_err[first + k] = static_cast<int8_t>(err);
+        if (used) {
+            const int32_t v = static_cast<int32_t>(mul_hi(exp_weight(d, sc), R) >> sh) - (1 << 30);
+            uint32_t rnd = 0;
+            if (p.round_mode == ROUND_STOCHASTIC) rnd = random_word(*p.seed, p.rng_stream, (p.rng_offset + row) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + mine);
+            one = one_entry(static_cast<int>(mine), narrow(v, 23, p.round_mode, rnd));
         }
-        if (lane == 0) p.row_stat[t] = make_int4(Mi, learns ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), one);
-        __syncwarp();
+        p.row_stat[row] = make_int4(M, used ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), one);
+        return;
+    }
+    // a teacher's entries: a warp to each row
+    const int i = warp, t = row0 + warp;
+    if (i >= RB || t >= p.rows) return;
+    unsigned long long Si = 0;
+    int32_t Mi = INT_MIN;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) { Si += s_sum[w][i]; Mi = max(Mi, s_max[w][i]); }
+    const int n = 32 - __clzll(static_cast<long long>(Si));
+    const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (Si >> n)), sh = static_cast<uint32_t>(n - 3);
+    const long long first = static_cast<long long>(t) * p.entries;
+    const int et = *p.exp_top - p.temperature;
+    const ExpScale st = exp_scale(et);
+    const auto teacher = [&](int k) {
+        return p.top32 ? static_cast<const int32_t*>(p.top)[first + k] : static_cast<int32_t>(static_cast<const int8_t*>(p.top)[first + k]);
+    };
+    // which entries there are, and the teacher's largest
+    bool any = false, wrong = false;
+    int32_t best = INT_MIN;
+    for (int k = lane; k < p.entries; k += 32) {
+        const long long j = p.index[first + k];
+        const bool used = j >= 0 && j < p.classes;
+        wrong |= j >= p.classes;
+        any |= used;
+        s_class[warp][k] = used ? static_cast<int>(j) : -1;
+        if (used) best = max(best, teacher(k));
+    }
+    any = __any_sync(0xFFFFFFFFu, any);
+    wrong = __any_sync(0xFFFFFFFFu, wrong);
+    best = __reduce_max_sync(0xFFFFFFFFu, best);
+    unsigned long long total = 0;
+    for (int k = lane; k < p.entries; k += 32) {
+        const unsigned share = s_class[warp][k] >= 0 ? exp_weight(static_cast<unsigned>(best) - static_cast<unsigned>(teacher(k)), st) : 0u;
+        s_share[warp][k] = share;
+        total += share;
+    }
+    total = warp_sum(total);
+    const double ln_s = log(static_cast<double>(Si) * pow2(-34)), ln_q = log(static_cast<double>(total) * pow2(-30)), teacher_unit = pow2(et);
+    double loss = 0.0;
+    for (int k = lane; k < p.entries; k += 32) {
+        const unsigned share = s_share[warp][k];
+        if (share == 0) continue;
+        const double lnp = -(static_cast<double>(static_cast<long long>(Mi) - p.logit[first + k]) * unit + ln_s);
+        const double lnq = -(static_cast<double>(static_cast<long long>(best) - teacher(k)) * teacher_unit + ln_q);
+        loss += static_cast<double>(share) / static_cast<double>(total) * (lnq - lnp);
+        s_share[warp][k] = static_cast<unsigned>((static_cast<unsigned long long>(share) << 30) / total);
+    }
+    loss = warp_sum(loss) * pow2(2 * p.temperature);
+    const bool learns = any && !wrong;
+    if (lane == 0) p.loss[t] = wrong ? __int_as_float(0x7FC00000) : any ? static_cast<float>(loss) : 0.0f;
+    if (p.row_stat == nullptr) return;
+    if (lane == 0) p.row_stat[t] = make_int4(Mi, learns ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), 0);
+    __syncwarp();
+    const unsigned long long seed = p.round_mode == ROUND_STOCHASTIC ? *p.seed : 0;
+    for (int k = lane; k < p.entries; k += 32) {
+        const int j = s_class[warp][k];
+        if (j < 0) continue;
+        int err = 0;
+        if (learns) {
+            unsigned q = 0;  // a class may be listed more than once
+            for (int o = 0; o < p.entries; ++o) q += s_class[warp][o] == j ? s_share[warp][o] : 0u;
+            const uint32_t E = exp_weight(static_cast<unsigned>(Mi) - static_cast<unsigned>(p.logit[first + k]), sc);
+            const int32_t v = static_cast<int32_t>(mul_hi(E, R) >> sh) - static_cast<int32_t>(q);
+            const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
+            err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
+        }
+        p.entry_err[first + k] = static_cast<int8_t>(err);
     }
 }
 
@@ -771,7 +813,111 @@ __global__ void __launch_bounds__(256) vocab_patch_kernel(const long long* index
     if (index[i] >= 0 && j >= 0 && j < count) err[(i / entries) * pitch + j] = entry_err[i];
 }
 
+// ---------------------------------------------------------------------------------------------- the error's narrowing
+struct NarrowParams {
+    const int32_t* e32; int F, F4, rows;      // [rows][F4], F of them written
+    int8_t* out;                              // [rows][F]
+    unsigned* max_word; int32_t* barrier;     // both zero before the first launch that finds the maximum
+    int find, narrow;                         // find: max |e32| into its word; narrow: by it.  Both: a cooperative launch
+    const int32_t* exp_a; const int32_t* exp_b; int32_t* exp_out;
+    int bits, mode;
+    const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
+    int32_t* status;
+};
+// err_calc (ti_torch.py:119-133) of an error that came in parts, so that nobody has seen its maximum yet.  A thread's first four words
+// stay in registers over the grid barrier: a small error is read once, and its two passes cost one launch (48 x 256: 6.3 us, two launches 4.2 + 4.7 and the way between them).
+constexpr int NARROW_HELD = 4;
+__global__ void __launch_bounds__(256) vocab_narrow_kernel(const NarrowParams p) {
+    __shared__ unsigned s_max[8];
+    __shared__ int s_flag;
+    const int tid = threadIdx.x, per_row = p.F4 / 4;
+    const bool dense = p.F4 == p.F;
+    const long long words = static_cast<long long>(p.rows) * per_row, step = static_cast<long long>(gridDim.x) * 256;
+    const long long first = static_cast<long long>(blockIdx.x) * 256 + tid;
+    const int4* src = reinterpret_cast<const int4*>(p.e32);
+    const auto load = [&](long long i) {
+        int4 v = __ldcg(src + i);
+        if (!dense) {
+            const int left = p.F - static_cast<int>(i % per_row) * 4;  // what lies behind a row is anything
+            if (left < 4) v.w = 0;
+            if (left < 3) v.z = 0;
+            if (left < 2) v.y = 0;
+        }
+        return v;
+    };
+    int4 held[NARROW_HELD];
+#pragma unroll
+    for (int u = 0; u < NARROW_HELD; ++u) held[u] = first + u * step < words ? load(first + u * step) : make_int4(0, 0, 0, 0);
+    if (p.find) {
+        unsigned m = 0;
+#pragma unroll
+        for (int u = 0; u < NARROW_HELD; ++u) m = max(m, absmax4(held[u]));
+        for (long long i = first + NARROW_HELD * step; i < words; i += step) m = max(m, absmax4(load(i)));
+        m = __reduce_max_sync(0xFFFFFFFFu, m);
+        if ((tid & 31) == 0) s_max[tid >> 5] = m;
+        __syncthreads();
+        if (tid == 0) {
+#pragma unroll
+            for (int w = 1; w < 8; ++w) m = max(m, s_max[w]);
+            if (m != 0) red_relaxed_max(p.max_word, m);
+        }
+        if (!p.narrow) return;
+        if (!bounded_grid_barrier(p.barrier, static_cast<int>(gridDim.x), p.status, 6, &s_flag)) return;
+    }
+    bool zero;
+    const int shift = shift_for(__ldcg(p.max_word), CALC_ERR, p.bits, &zero);
+    if (blockIdx.x == 0 && tid == 0) *p.exp_out = shift + *p.exp_a + *p.exp_b;
+    const bool stochastic = p.mode == ROUND_STOCHASTIC && shift > 0;
+    const unsigned long long seed = stochastic ? *p.seed : 0;
+    const auto emit = [&](long long i, const int4& v) {
+        const int x[4] = {v.x, v.y, v.z, v.w};
+        if (dense) {
+            uint32_t rnd[4] = {0, 0, 0, 0}, o = 0;
+            if (stochastic) random_block(seed, p.rng_stream, (p.rng_offset >> 2) + i, rnd);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o |= static_cast<uint32_t>(static_cast<uint8_t>(narrow(x[j], shift, p.mode, rnd[j]))) << (8 * j);
+            reinterpret_cast<uint32_t*>(p.out)[i] = o;
+        } else {
+            const long long row = i / per_row;
+            const int f = static_cast<int>(i - row * per_row) * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (f + j < p.F) {
+                    const long long at = row * p.F + f + j;
+                    p.out[at] = narrow(x[j], shift, p.mode, stochastic ? random_word(seed, p.rng_stream, p.rng_offset + at) : 0u);
+                }
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < NARROW_HELD; ++u) if (first + u * step < words) emit(first + u * step, held[u]);
+#pragma unroll 2
+    for (long long i = first + NARROW_HELD * step; i < words; i += step) emit(i, load(i));
+}
+
 // ---------------------------------------------------------------------------------------------- host side
+// err_calc of the whole error; `summed`: its maximum is still to be found
+int narrow_error(NarrowParams p, bool summed, cudaStream_t st) {
+    const long long words = static_cast<long long>(p.rows) * (p.F4 / 4), blocks = (words + 1023) / 1024, most = 4ll * sm_count();
+    const unsigned grid = static_cast<unsigned>(blocks < 1 ? 1 : blocks < most ? blocks : most);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(256); cfg.stream = st;
+    if (summed && g_cooperative) {
+        p.find = p.narrow = 1;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeCooperative; attr[0].val.cooperative = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        const int e = launched_together(cudaLaunchKernelEx(&cfg, vocab_narrow_kernel, p));
+        if (e != LAUNCH_REFUSED) return e;
+        cfg.numAttrs = 0;
+    }
+    if (summed) {
+        p.find = 1; p.narrow = 0;
+        if (int e = launched(cudaLaunchKernelEx(&cfg, vocab_narrow_kernel, p))) return e;
+    }
+    p.find = 0; p.narrow = 1;
+    return launched(cudaLaunchKernelEx(&cfg, vocab_narrow_kernel, p));
+}
+
 template <bool TWO, int WHAT, int BN>
 int launch_vocab_inst(const CUtensorMap& a, const CUtensorMap& b, const VocabParams& p, cudaStream_t st) {
     using Cfg = VocabCfg<TWO, BN>;
@@ -882,7 +1028,7 @@ VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
         p.entry_at = take(t * k);
         p.err_at = take(t * p.piece);
         p.e32_at = take(4 * t * up(F, 4));
-        if (F % 4 != 0) p.g32_at = take(4 * up(F, 4) * (static_cast<size_t>(p.piece) > t ? p.piece : t));
+        if (F % 4 != 0) p.g32_at = take(4 * up(F, 4) * static_cast<size_t>(p.piece));
     }
     p.bytes = at;
     return p;
@@ -954,7 +1100,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     } else if (int e = run_vocab(VOCAB_STATS, x, w, T, F, pl.pitch, V, &vp, a->status, st)) {
         return e;
     }
-    if (K > 1 && !thin) {
+    if (a->top != nullptr && !thin) {
         const EntryParams ep{x, w, pl.pitch / 16, T, V, K, index, logit};
         const long long warps = static_cast<long long>(T) * ((K + ENTRIES_PER_WARP - 1) / ENTRIES_PER_WARP);
         vocab_entries_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, st>>>(ep);
@@ -967,8 +1113,8 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     fp.rows_log2 = T >= 1024 ? 3 : T >= 256 ? 2 : 0;  // eight words of a piece fill a sector; few rows are better off in blocks of their own
     fp.piece_max = vp.piece_max; fp.piece_sum = vp.piece_sum;
     fp.index = index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = logit; fp.loss = a->loss;
-    if (K == 1 && !thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
-    int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|}
+    if (a->top == nullptr && !thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
+    int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|, barrier}
     // e32 (+)= err w and g32 = err^T x of a piece of the vocabulary
     const int F4 = static_cast<int>(up(F, 4));
     int32_t* e32 = reinterpret_cast<int32_t*>(ws + pl.e32_at);
@@ -989,13 +1135,14 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     if (train) {
         fp.row_stat = reinterpret_cast<int4*>(ws + pl.stat_at);
         fp.entry_err = reinterpret_cast<int8_t*>(ws + pl.entry_at);
-        fp.err_exp = words; fp.clear[0] = reinterpret_cast<uint32_t*>(words + 1); fp.clear[1] = a->grad_maxabs;
+        fp.err_exp = words; fp.clear[0] = reinterpret_cast<uint32_t*>(words + 1); fp.clear[1] = reinterpret_cast<uint32_t*>(words + 2); fp.clear[2] = a->grad_maxabs;
         if (plan.splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
         fp.round_mode = a->loss_round;
         fp.seed = reinterpret_cast<const unsigned long long*>(a->seed); fp.rng_stream = a->loss_stream; fp.rng_offset = a->sample_offset;
     }
     const int rb = 1 << fp.rows_log2;
-    vocab_finish_kernel<<<(T + rb - 1) / rb, FINISH_THREADS, 0, st>>>(fp);
+    if (a->top == nullptr) vocab_finish_kernel<true><<<(T + rb - 1) / rb, FINISH_THREADS, 0, st>>>(fp);
+    else                   vocab_finish_kernel<false><<<(T + rb - 1) / rb, FINISH_THREADS, 0, st>>>(fp);
     if (int e = launched(cudaGetLastError())) return e;
     if (!train) return NITI_OK;
 
@@ -1006,7 +1153,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
         vp.first = v0;
         if (int e = run_vocab(a->loss_round, x, w, T, F, pl.pitch, count, &vp, a->status, st)) return e;
-        if (K > 1) {
+        if (a->top != nullptr) {
             vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(index, fp.entry_err, wanted, K, v0, count, vp.err, vp.err_pitch);
             if (int e = launched(cudaGetLastError())) return e;
         }
@@ -1015,12 +1162,12 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         if (F % 4 != 0)
             if (int e = copy_rows(to_w.out, 4ll * F4, a->g32 + static_cast<long long>(v0) * F, 4ll * F, 4ll * F, count, 4, st)) return e;
     }
-    int32_t* dense = e32;
-    if (F4 != F) {
-        dense = reinterpret_cast<int32_t*>(ws + pl.g32_at);
-        if (int e = copy_rows(e32, 4ll * F4, dense, 4ll * F, 4ll * F, T, 4, st)) return e;
-    }
-    if (summed) if (int e = absmax_i32(dense, static_cast<long long>(T) * F, e32_max, st)) return e;
-    return niti_requant_i8(dense, a->e8, e32_max, static_cast<long long>(T) * F, NITI_CALC_ERR, a->bits, a->err_round, a->seed, a->err_stream,
-                           a->sample_offset * static_cast<uint64_t>(F), 0, words, a->exp_w, a->exp_err, nullptr, stream);
+    NarrowParams np{};
+    np.e32 = e32; np.F = F; np.F4 = F4; np.rows = T; np.out = a->e8;
+    np.max_word = e32_max; np.barrier = words + 2;
+    np.exp_a = words; np.exp_b = a->exp_w; np.exp_out = a->exp_err;
+    np.bits = a->bits; np.mode = a->err_round;
+    np.seed = fp.seed; np.rng_stream = a->err_stream; np.rng_offset = a->sample_offset * static_cast<unsigned long long>(F);
+    np.status = a->status;
+    return narrow_error(np, summed, st);
 }

@@ -69,8 +69,8 @@ def vocab(x, exp_x, w, exp_w, index, ignore_index=-100, top=None, exp_top=0, tem
     learns = np.zeros(T, dtype=bool)
     want = np.zeros((T, V), dtype=np.int64)
     for t in range(T):
-        used = [k for k, j in enumerate(index[t]) if 0 <= j < V]
-        if any(j >= V or (top is None and j < 0 and j != ignore_index) for j in index[t]):
+        used = [k for k, j in enumerate(index[t]) if 0 <= j < V and (top is not None or j != ignore_index)]
+        if any((j >= V or (top is None and j < 0)) and (top is not None or j != ignore_index) for j in index[t]):
             loss[t] = math.nan
             continue
         if not used:

@@ -135,6 +135,30 @@ def test_rows_without_a_class():
     check_train((loss, e8, exp_err, g32, gmax), want)
 
 
+@pytest.mark.parametrize("ignore", [0, 5, 599, 600, 2 ** 33, -7])
+def test_any_class_can_be_the_one_to_ignore(ignore):
+    T, F, V = 150, 48, 600
+    rng, x, ex, w, ew, y = layer(14, T, F, V)
+    y[rng.random(T) < 0.3] = ignore
+    want = VO.vocab(x, ex, w, ew, y, ignore_index=ignore)
+    assert (want["loss"] == 0).any()
+    check_train(ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y), ignore), want)
+    same_loss(ops.vocab_loss(cu(x[:3]), word(ex), cu(w), word(ew), cu(y[:3]), ignore), want["loss"][:3])
+
+
+def test_plain_launches_give_the_same():
+    """Where cooperative launches are off, the error's maximum and its narrowing are two launches."""
+    for T, F, V in ((300, 320, 3000), (40, 30, 2000)):
+        rng, x, ex, w, ew, y = layer(16, T, F, V)
+        a = ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y))
+        old = ops.set_cooperative_launch(False)
+        try:
+            b = ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y))
+        finally:
+            ops.set_cooperative_launch(old)
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 def test_no_tokens():
     w, ew = cu(np.ones((70, 16), np.int8)), word(-3)
     x = torch.empty((0, 16), dtype=torch.int8, device=DEV)
