@@ -623,6 +623,21 @@ PyObject* vocab_loss(Args& a) {
     TORCH_CHECK(seed == nullptr || (seed->scalar_type() == at::kLong && seed->numel() >= 1), "niti_b200 vocab ops: the seed is one int64");
     TORCH_CHECK(g32 == nullptr || (g32->scalar_type() == at::kInt && g32->sizes() == w.sizes()), "niti_b200 vocab ops: g32 is int32 of the weights' shape");
     const int64_t T = x.size(0), F = x.size(1), V = w.size(0), K = top ? index.size(1) : 1;
+    if (T == 0 && w.size(0) > 0) {  // nothing to learn: the same shapes
+        Tensor loss, e8, exp_err, g, gmax;
+        {
+            Launch l(x);
+            loss = l.empty({0}, at::kFloat);
+            if (train) {
+                e8 = l.empty({0, F}, at::kChar);
+                exp_err = exp_w.reshape({}) + (temperature - 7);
+                g = g32 ? *g32 : l.empty({V, F}, at::kInt);
+                g.zero_();
+                gmax = at::zeros({1}, exp_w.options());
+            }
+        }
+        return train ? tuple(loss, e8, exp_err, g, gmax) : wrap(loss);
+    }
     TORCH_CHECK(T < (1ll << 31) && F < (1ll << 31) && V < (1ll << 31) && K < (1ll << 31) && niti_vocab_supported(int(T), int(F), int(V), int(K)),
                 "niti_b200 vocab ops: 1 to 131071 tokens and features, 1 to 262144 classes and 1 to 128 entries are supported: got ", T, ", ", F, ", ", V, ", ", K);
     Tensor loss, e8, exp_err, gmax, g;

@@ -98,6 +98,7 @@ struct GemmParams {
     int group_m;           // GEMM tile order: row tiles per group (0 / 1: plain row-major)
     int nstages;           // stages of the ring actually used (<= the compiled maximum; tuning / experiments)
     int accumulate;        // plain products: tiles are added to the result
+    int32_t* plain_out;    // plain products: the result [M][N] where its rows are no whole 16-byte groups (null: through the tensor map)
     int split_cols;        // 1: both epilogue warpgroups share every tile (alternate 128-column groups); 0: they alternate tiles
     // fused requantisation (FUSED kernels): int8 output narrowed by the shift in state[0].
     // state = {shift, max|acc|, redo flag, redo count, finished-CTA ticket}; the last CTA of a first

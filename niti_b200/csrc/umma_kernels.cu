@@ -388,7 +388,9 @@ __device__ __forceinline__ void store_piece(int8_t* at, int cols, const uint32_t
 }
 
 // Plain products: int32 out (+ max|acc|).  cta_first, cta_step: the tiles of this thread block (of a pair of them)
-template <int BN, bool TWO, bool ROWS32>
+// PLAIN: a result whose rows are no whole 16-byte groups (p.plain_out) leaves the staging tiles by ordinary stores, a row's 64 columns
+// to a warp at a time (918 x 1426, 40001 classes: 113 us; through a padded copy 113 + 147).
+template <int BN, bool TWO, bool ROWS32, bool PLAIN = false>
 __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const GemmParams& p,
                                           const int cta_first, const int cta_step) {
     using Cfg = GemmCfg<BN, TWO>;
@@ -543,7 +545,18 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
                     stage_row(buf + EPI_CHUNK_BYTES, row_in_tile, v[2 * half_i + 1]);
                     fence_proxy_async();
                     named_barrier(bar_id, 128);
-                    if (leader) {
+                    if (PLAIN && p.plain_out != nullptr) {
+                        const int cx = col0 + g0 + half_i * 64;
+#pragma unroll 4
+                        for (int r = q; r < min(128, p.M - cy); r += 4) {
+                            int32_t* to = p.plain_out + static_cast<long long>(cy + r) * p.N + cx;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t at = buf + h * EPI_CHUNK_BYTES + static_cast<uint32_t>(r) * 128u + (static_cast<uint32_t>((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+                                if (cx + h * 32 + lane < p.N) to[h * 32 + lane] = static_cast<int32_t>(ld_shared_u32(at));
+                            }
+                        }
+                    } else if (leader) {
                         const int cx = col0 + g0 + half_i * 64;
                         if (p.accumulate) {
                             tma_reduce_add_4d(&tmC, buf, cx, cy, cz, cw);
@@ -601,12 +614,12 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 // Two products in one launch, the first `units` thread blocks (pairs of them) at one and the others at the other.
 struct GemmTwoMaps { CUtensorMap a[2], b[2], c[2]; };
 struct GemmTwoParams { GemmParams job[2]; int units; };
-template <int BN, bool TWO>
+template <int BN, bool TWO, bool PLAIN>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 umma_gemm_two_kernel(const __grid_constant__ GemmTwoMaps maps, const __grid_constant__ GemmTwoParams tp) {
     const int unit = static_cast<int>(TWO ? blockIdx.x >> 1 : blockIdx.x), all = static_cast<int>(TWO ? gridDim.x >> 1 : gridDim.x);
     const int j = unit >= tp.units ? 1 : 0;
-    gemm_body<BN, TWO, false>(maps.a[j], maps.b[j], maps.c[j], tp.job[j], j ? unit - tp.units : unit, j ? all - tp.units : tp.units);
+    gemm_body<BN, TWO, false, PLAIN>(maps.a[j], maps.b[j], maps.c[j], tp.job[j], j ? unit - tp.units : unit, j ? all - tp.units : tp.units);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -2109,6 +2122,8 @@ static int gemm_setup(const GemmCall& g, int bn, bool pair, bool int32_out, Gemm
     const uint64_t results = g.accumulate ? 1 : g.splits;
     uint64_t dc[4] = {(uint64_t)g.N, (uint64_t)g.M, results, 1};
     const uint64_t pitch = g.ldc > 0 ? g.ldc : g.N;
+    p->plain_out = pitch % 4 != 0 ? static_cast<int32_t*>(g.out) : nullptr;  // rows a tensor map cannot describe (umma_gemm_two alone)
+    if (p->plain_out != nullptr) int32_out = false;
     uint64_t sc[3] = {pitch * 4, g.M * pitch * 4, results * g.M * pitch * 4};
     uint32_t bc[4] = {32, 128, 1, 1};
     if (int32_out) if (int e = encode_map(&m->c, g.out, true, 4, dc, sc, bc)) return e;
@@ -2180,10 +2195,10 @@ GemmTwoPlan umma_gemm_two_plan(const GemmCall& first, const GemmCall& second) {
     }
     return best;
 }
-template <int BN, bool TWO>
+template <int BN, bool TWO, bool PLAIN>
 static int launch_gemm_two(const GemmTwoMaps& maps, const GemmTwoParams& tp, int grid, cudaStream_t st) {
     using Cfg = GemmCfg<BN, TWO>;
-    cudaError_t e = allow_shared<umma_gemm_two_kernel<BN, TWO>>(Cfg::SMEM_BYTES);
+    cudaError_t e = allow_shared<umma_gemm_two_kernel<BN, TWO, PLAIN>>(Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return set_cuda_error(e);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(GEMM_THREADS); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
@@ -2191,7 +2206,7 @@ static int launch_gemm_two(const GemmTwoMaps& maps, const GemmTwoParams& tp, int
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = TWO ? 1 : 0;
-    return launched(cudaLaunchKernelEx(&cfg, umma_gemm_two_kernel<BN, TWO>, maps, tp));
+    return launched(cudaLaunchKernelEx(&cfg, umma_gemm_two_kernel<BN, TWO, PLAIN>, maps, tp));
 }
 int umma_gemm_two(const GemmCall& first, const GemmCall& second, const GemmTwoPlan& plan, cudaStream_t st) {
     GemmTwoMaps maps;
@@ -2200,7 +2215,7 @@ int umma_gemm_two(const GemmCall& first, const GemmCall& second, const GemmTwoPl
     for (int j = 0; j < 2; ++j) {
         GemmCall g = j ? second : first;
         if (!j) g.splits = plan.splits;
-        GemmMaps m;
+        GemmMaps m{};
         if (int e = gemm_setup(g, plan.bn, plan.pair, true, &m, &tp.job[j])) return e;
         maps.a[j] = m.a; maps.b[j] = m.b; maps.c[j] = m.c;
         GemmParams& p = tp.job[j];
@@ -2209,8 +2224,11 @@ int umma_gemm_two(const GemmCall& first, const GemmCall& second, const GemmTwoPl
         set_fused(&p, nullptr);
         finish_params(&p);
     }
-    return plan.bn == 256 ? (plan.pair ? launch_gemm_two<256, true>(maps, tp, plan.grid, st) : launch_gemm_two<256, false>(maps, tp, plan.grid, st))
-                          : launch_gemm_two<128, false>(maps, tp, plan.grid, st);
+    if (tp.job[0].plain_out != nullptr || tp.job[1].plain_out != nullptr)
+        return plan.bn == 256 ? (plan.pair ? launch_gemm_two<256, true, true>(maps, tp, plan.grid, st) : launch_gemm_two<256, false, true>(maps, tp, plan.grid, st))
+                              : launch_gemm_two<128, false, true>(maps, tp, plan.grid, st);
+    return plan.bn == 256 ? (plan.pair ? launch_gemm_two<256, true, false>(maps, tp, plan.grid, st) : launch_gemm_two<256, false, false>(maps, tp, plan.grid, st))
+                          : launch_gemm_two<128, false, false>(maps, tp, plan.grid, st);
 }
 
 // Forward convolution (flip == 0: x [N,H,W,C] with w [K,R,S,C] -> [N,H,W,K]) or error-backward

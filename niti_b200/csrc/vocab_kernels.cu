@@ -99,6 +99,7 @@ struct VocabParams {
     int rows;                 // tokens
     int first, classes;       // of the piece of the vocabulary this launch covers (multiple of 256); classes of the whole vocabulary
     int32_t* piece_max; uint32_t* piece_sum;  // [pieces][rows]
+    const int* entries; int num_entries;      // a teacher's classes and their errors (one_entry), [num_entries][rows]; 0: none, or vocab_patch_kernel's
     const int4* row_stat;     // {M, R, n - 3, the wanted class where there is one: see one_entry}; R = 0: a row without an error
     int8_t* err; long long err_pitch;
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
@@ -111,7 +112,8 @@ struct VocabCfg {
     static constexpr int BLOCKS = TWO ? 2 : 1;  // 128-byte reduction blocks of a stage
     static constexpr int B_PANEL_BYTES = (TWO ? BN / 2 : BN) * ROW_BYTES;
     static constexpr int STAGE_BYTES = BLOCKS * (PANEL_BYTES + B_PANEL_BYTES);
-    static constexpr int STAGES = 224 * 1024 / STAGE_BYTES;
+    static constexpr int PER_SM = BN == 64 ? 3 : 1;  // thread blocks
+    static constexpr int STAGES = 224 * 1024 / PER_SM / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
 };
 
@@ -272,7 +274,7 @@ enum { VOCAB_STATS = 3 };  // beside the three roundings of the error kernel
 // epilogue warps (sixteen for 256 columns) take a tile's 64-column groups out of tensor memory into registers, hand the accumulator
 // back at once and work on the registers under the next tile's MMAs.
 template <bool TWO, int WHAT, int BN>
-__global__ void __launch_bounds__(vocab_threads(BN), 1)
+__global__ void __launch_bounds__(vocab_threads(BN), (VocabCfg<TWO, BN>::PER_SM))
 vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const VocabParams vp) {
     using Cfg = VocabCfg<TWO, BN>;
     constexpr int STAGES = Cfg::STAGES;
@@ -387,6 +389,11 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 }
                 const int at = (stat.w & 0x3FFFF) - vp.first - col;
                 if ((stat.w & (1 << 23)) && at >= 0 && at < PIECE) out[at] = static_cast<int8_t>(stat.w >> 24);
+#pragma unroll 4
+                for (int k = 0; k < vp.num_entries; ++k) {
+                    const int w = __ldg(vp.entries + static_cast<long long>(k) * vp.rows + row), to = (w & 0x3FFFF) - vp.first - col;
+                    if ((w & (1 << 23)) && to >= 0 && to < PIECE) out[to] = static_cast<int8_t>(w >> 24);
+                }
             }
         }
     }
@@ -405,9 +412,15 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 // ---------------------------------------------------------------------------------------------- operands of odd rows
 // Rows of `bytes` bytes, one behind the other from any address, to rows of a pitch of 16 bytes, the rest of each zeroed.  A thread to
 // 16 bytes: five aligned words and four funnel shifts; what lies across the tensor's ends is read byte by byte.
-__global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restrict__ src, uint4* __restrict__ dst, int bytes, int pitch16, long long pieces, long long total) {
-    const uintptr_t begin = reinterpret_cast<uintptr_t>(src), end = begin + total;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces; i += static_cast<long long>(gridDim.x) * 256) {
+// Two tensors with rows of the same length in one launch.
+__global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restrict__ src0, long long rows0, const int8_t* __restrict__ src1, long long rows1,
+                                                          uint4* __restrict__ dst0, uint4* __restrict__ dst1, int bytes, int pitch16) {
+    const long long pieces0 = rows0 * pitch16, pieces = pieces0 + rows1 * pitch16;
+    for (long long n0 = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; n0 < pieces; n0 += static_cast<long long>(gridDim.x) * 256) {
+        const bool second = n0 >= pieces0;
+        const long long i = second ? n0 - pieces0 : n0;
+        const int8_t* const src = second ? src1 : src0;
+        const uintptr_t begin = reinterpret_cast<uintptr_t>(src), end = begin + (second ? rows1 : rows0) * bytes;
         const long long row = i / pitch16;
         const int c = static_cast<int>(i - row * pitch16) * 16, n = min(16, bytes - c);
         const uintptr_t at = begin + row * bytes + c, word0 = at & ~uintptr_t(3);
@@ -434,12 +447,12 @@ __global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restri
             const int left = n - 4 * k;
             if (left < 4) o[k] = left <= 0 ? 0u : o[k] & ((1u << (8 * left)) - 1u);
         }
-        dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        (second ? dst1 : dst0)[i] = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
-int align_rows(const int8_t* src, void* dst, int bytes, int pitch, long long rows, cudaStream_t st) {
-    const long long pieces = rows * (pitch / 16), blocks = (pieces + 255) / 256, most = 16ll * sm_count();
-    vocab_align_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, st>>>(src, static_cast<uint4*>(dst), bytes, pitch / 16, pieces, rows * bytes);
+int align_rows(const int8_t* src0, long long rows0, void* dst0, const int8_t* src1, long long rows1, void* dst1, int bytes, int pitch, cudaStream_t st) {
+    const long long blocks = ((rows0 + rows1) * (pitch / 16) + 255) / 256, most = 16ll * sm_count();
+    vocab_align_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, st>>>(src0, rows0, src1, rows1, static_cast<uint4*>(dst0), static_cast<uint4*>(dst1), bytes, pitch / 16);
     return launched(cudaGetLastError());
 }
 
@@ -618,7 +631,7 @@ struct FinishParams {
     int32_t* logit;                            // of the wanted classes; of a single one per row it is computed here
     const int8_t* x; const int8_t* w; int F16; // null: they are all there
     float* loss;
-    int4* row_stat; int8_t* entry_err;         // null: the loss alone
+    int4* row_stat; int* entry_err;            // null: the loss alone; entry_err [entries][rows], see one_entry
     int32_t* err_exp; uint32_t* clear[3];      // training: written and zeroed for the launches behind
     uint4* zero; long long zero_count;         // training: zeroed as well
     int round_mode;
@@ -729,7 +742,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
         if (used) {
             const int32_t v = static_cast<int32_t>(mul_hi(exp_weight(d, sc), R) >> sh) - (1 << 30);
             uint32_t rnd = 0;
-            if (p.round_mode == ROUND_STOCHASTIC) rnd = random_word(*p.seed, p.rng_stream, (p.rng_offset + row) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + mine);
+            if (p.round_mode == ROUND_STOCHASTIC) rnd = random_word(*p.seed, p.rng_stream, (p.rng_offset + row) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + static_cast<unsigned long long>(mine));
             one = one_entry(static_cast<int>(mine), narrow(v, 23, p.round_mode, rnd));
         }
         p.row_stat[row] = make_int4(M, used ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), one);
@@ -790,7 +803,8 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     const unsigned long long seed = p.round_mode == ROUND_STOCHASTIC ? *p.seed : 0;
     for (int k = lane; k < p.entries; k += 32) {
         const int j = s_class[warp][k];
-        if (j < 0) continue;
+        int& out = p.entry_err[static_cast<long long>(k) * p.rows + t];
+        if (j < 0) { out = 0; continue; }
         int err = 0;
         if (learns) {
             unsigned q = 0;  // a class may be listed more than once
@@ -800,17 +814,16 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
             const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
             err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
         }
-        p.entry_err[first + k] = static_cast<int8_t>(err);
+        out = one_entry(j, err);
     }
 }
 
-// the errors of the wanted classes of a piece of the vocabulary, over what vocab_kernel wrote there
-__global__ void __launch_bounds__(256) vocab_patch_kernel(const long long* index, const int8_t* entry_err, long long n, int entries, int first, int count,
-                                                          int8_t* err, long long pitch) {
+// a teacher's entries in a piece of the vocabulary, over what vocab_kernel wrote there
+__global__ void __launch_bounds__(256) vocab_patch_kernel(const int* entries, long long n, int rows, int first, int count, int8_t* err, long long pitch) {
     const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= n) return;
-    const long long j = index[i] - first;
-    if (index[i] >= 0 && j >= 0 && j < count) err[(i / entries) * pitch + j] = entry_err[i];
+    const int w = entries[i], j = (w & 0x3FFFF) - first;
+    if ((w & (1 << 23)) && j >= 0 && j < count) err[(i % rows) * pitch + j] = static_cast<int8_t>(w >> 24);
 }
 
 // ---------------------------------------------------------------------------------------------- the error's narrowing
@@ -923,7 +936,7 @@ int launch_vocab_inst(const CUtensorMap& a, const CUtensorMap& b, const VocabPar
     using Cfg = VocabCfg<TWO, BN>;
     cudaError_t e = allow_shared<vocab_kernel<TWO, WHAT, BN>>(Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return set_cuda_error(e);
-    const int units = sm_count() / (TWO ? 2 : 1), tiles = p.g.m_tiles * p.g.n_tiles, grid = tiles < units ? tiles : units;
+    const int units = sm_count() * Cfg::PER_SM / (TWO ? 2 : 1), tiles = p.g.m_tiles * p.g.n_tiles, grid = tiles < units ? tiles : units;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(vocab_threads(BN)); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -941,13 +954,28 @@ int launch_vocab(int what, const CUtensorMap& a, const CUtensorMap& b, const Voc
         default: return launch_vocab_inst<TWO, VOCAB_STATS, BN>(a, b, p, st);
     }
 }
+// The tile of a launch: 256 columns of 128 rows (or of 256, to a pair of thread blocks), or 64 columns in up to three thread blocks to an SM,
+// for launches whose last wave of wide tiles would be far from full.  Cycles: an epilogue of 256 columns, one and two of 64 on an SM; a
+// 128-byte reduction block of each; the first tile's blocks lie in front of every epilogue.  48 x 256 x 4096 (64 SMs instead of
+// 16): 11.8 -> 8.2 us; 333 x 640 x 20011 (939 tiles of 64 instead of three waves of pairs), the loss: 28.7 -> 22.6 us.
+struct VocabTile { int bn; bool pair; };
+VocabTile vocab_tile(int m128, int F, int count) {
+    const long long kb = (F + 127) / 128, sms = sm_count();
+    const bool pair = (g_two_cta & 1) && m128 >= 2;
+    const auto larger = [](long long a, long long b) { return a > b ? a : b; };
+    const long long wide = static_cast<long long>(pair ? (m128 + 1) / 2 : m128) * ((count + VBN - 1) / VBN), units = pair ? sms / 2 : sms, block = pair ? 600 : 700;
+    const long long wide_cost = kb * block + (wide + units - 1) / units * larger(10400, kb * block);
+    const long long narrow = static_cast<long long>(m128) * ((count + 63) / 64), whole = narrow / (2 * sms), rest = narrow - whole * 2 * sms;
+    const long long full = larger(5400, 2 * kb * 650), last = rest == 0 ? 0 : rest <= sms ? larger(4200, kb * 400) : full;
+    const long long narrow_cost = kb * 400 + whole * full + last;
+    return narrow_cost < wide_cost ? VocabTile{64, false} : VocabTile{VBN, pair};
+}
 // x [T][pitch] times `count` rows of w [V][pitch] from p->first on
 int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitch, int count, VocabParams* p, int32_t* status, cudaStream_t st) {
-    // A tile's 64-column groups share the SM's integer pipes: where all tiles of 64 or 128 columns find an SM of their own, a tile of 256
-    // takes longer (48 x 256 x 4096, 64 SMs instead of 16: the launch 11.8 -> 8.2 us).
     const int m128 = (T + 127) / 128;
-    const int bn = m128 * ((count + 63) / 64) <= sm_count() ? 64 : m128 * ((count + 127) / 128) <= sm_count() ? 128 : VBN;
-    const bool pair = (g_two_cta & 1) && m128 >= 2 && bn == VBN;
+    const VocabTile tile = vocab_tile(m128, F, count);
+    const int bn = tile.bn;
+    const bool pair = tile.pair;
     CUtensorMap ma, mb;
     uint64_t dims[2] = {static_cast<uint64_t>(F), static_cast<uint64_t>(T)}, str[1] = {static_cast<uint64_t>(pitch)};
     uint32_t box[2] = {128, 128};
@@ -962,7 +990,7 @@ int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitc
     g.group_m = (static_cast<long long>(T) + count) * F > (48ll << 20) ? 8 : 0;  // as umma_gemm orders its tiles
     g.fd_mn = make_fastdiv(g.m_tiles * g.n_tiles); g.fd_n = make_fastdiv(g.n_tiles); g.fd_tw = make_fastdiv(1); g.fd_th = make_fastdiv(1);
     if (pair) return launch_vocab<true, VBN>(what, ma, mb, *p, st);
-    return bn == 64 ? launch_vocab<false, 64>(what, ma, mb, *p, st) : bn == 128 ? launch_vocab<false, 128>(what, ma, mb, *p, st) : launch_vocab<false, VBN>(what, ma, mb, *p, st);
+    return bn == 64 ? launch_vocab<false, 64>(what, ma, mb, *p, st) : launch_vocab<false, VBN>(what, ma, mb, *p, st);
 }
 
 size_t up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -998,7 +1026,7 @@ int launch_thin(int T, const ThinParams& p, size_t smem, cudaStream_t st) {
 // The workspace of a call.
 struct VocabPlan {
     int pieces, pitch, piece;   // row pitch of the operands; classes whose errors are in the workspace at a time
-    size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, g32_at, bytes;
+    size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, bytes;
 };
 // Errors in the workspace at a time.  Pieces of 37 column tiles: 148 SMs are 74 pairs of thread blocks, so the errors' tiles and the weight
 // gradient's come in whole waves where the tokens, or the features, fill an even number of 256-row tiles.
@@ -1025,10 +1053,9 @@ VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     if (p.pitch != F && (train || !thin_serves(T, F))) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
     if (train) {
         p.stat_at = take(16 * t);
-        p.entry_at = take(t * k);
+        p.entry_at = take(4 * t * k);
         p.err_at = take(t * p.piece);
         p.e32_at = take(4 * t * up(F, 4));
-        if (F % 4 != 0) p.g32_at = take(4 * up(F, 4) * static_cast<size_t>(p.piece));
     }
     p.bytes = at;
     return p;
@@ -1076,8 +1103,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     if (pl.pitch != F && (train || !thin)) {
         x = reinterpret_cast<int8_t*>(ws + pl.x_at);
         w = reinterpret_cast<int8_t*>(ws + pl.w_at);
-        if (int e = align_rows(a->x, ws + pl.x_at, F, pl.pitch, T, st)) return e;
-        if (int e = align_rows(a->w, ws + pl.w_at, F, pl.pitch, V, st)) return e;
+        if (int e = align_rows(a->x, T, ws + pl.x_at, a->w, V, ws + pl.w_at, F, pl.pitch, st)) return e;
     } else if (pl.pitch == F && (!aligned16(x) || !aligned16(w))) {
         return NITI_ERR_BAD_ARG;
     }
@@ -1122,9 +1148,8 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     int8_t* err = reinterpret_cast<int8_t*>(ws + pl.err_at);
     GemmCall to_x{}, to_w{};
     const auto piece_calls = [&](int v0, int count) {
-        int32_t* g = F % 4 == 0 ? a->g32 + static_cast<long long>(v0) * F : reinterpret_cast<int32_t*>(ws + pl.g32_at);
         to_x = GemmCall{err, w + static_cast<long long>(v0) * pl.pitch, e32, e32_max, T, F, count, 0, 0, 1, pl.piece, pl.pitch, F4, v0 > 0, a->status};
-        to_w = GemmCall{err, x, g, a->grad_maxabs, count, F, T, 1, 0, 1, pl.piece, pl.pitch, F4, 0, a->status};
+        to_w = GemmCall{err, x, a->g32 + static_cast<long long>(v0) * F, a->grad_maxabs, count, F, T, 1, 0, 1, pl.piece, pl.pitch, F, 0, a->status};
         const GemmTwoPlan plan = umma_gemm_two_plan(to_x, to_w);
         if (plan.splits > 1) to_x.accumulate = 1;
         return plan;
@@ -1134,7 +1159,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     const bool summed = train && (plan.splits > 1 || pl.piece < V);  // e32 comes in several parts
     if (train) {
         fp.row_stat = reinterpret_cast<int4*>(ws + pl.stat_at);
-        fp.entry_err = reinterpret_cast<int8_t*>(ws + pl.entry_at);
+        fp.entry_err = reinterpret_cast<int*>(ws + pl.entry_at);
         fp.err_exp = words; fp.clear[0] = reinterpret_cast<uint32_t*>(words + 1); fp.clear[1] = reinterpret_cast<uint32_t*>(words + 2); fp.clear[2] = a->grad_maxabs;
         if (plan.splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
         fp.round_mode = a->loss_round;
@@ -1148,19 +1173,21 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
 
     vp.row_stat = fp.row_stat;
     vp.err = err; vp.err_pitch = pl.piece;
+    // A teacher's entries are looked through by every piece of a row (about three operations each beside some twenty for each of its 64
+    // classes), or written by a launch of their own, 4 us a piece of the vocabulary: even at about 2^30 rows x classes x entries.
+    const bool patch = a->top != nullptr && static_cast<long long>(T) * pl.piece * K > (1ll << 30);
+    if (a->top != nullptr && !patch) { vp.entries = fp.entry_err; vp.num_entries = K; }
     vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
     for (int v0 = 0; v0 < V; v0 += pl.piece) {
         const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
         vp.first = v0;
         if (int e = run_vocab(a->loss_round, x, w, T, F, pl.pitch, count, &vp, a->status, st)) return e;
-        if (a->top != nullptr) {
-            vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(index, fp.entry_err, wanted, K, v0, count, vp.err, vp.err_pitch);
+        if (patch) {
+            vocab_patch_kernel<<<static_cast<unsigned>((wanted + 255) / 256), 256, 0, st>>>(fp.entry_err, wanted, T, v0, count, vp.err, vp.err_pitch);
             if (int e = launched(cudaGetLastError())) return e;
         }
         if (v0 > 0) plan = piece_calls(v0, count);
         if (int e = umma_gemm_two(to_x, to_w, plan, st)) return e;
-        if (F % 4 != 0)
-            if (int e = copy_rows(to_w.out, 4ll * F4, a->g32 + static_cast<long long>(v0) * F, 4ll * F, 4ll * F, count, 4, st)) return e;
     }
     NarrowParams np{};
     np.e32 = e32; np.F = F; np.F4 = F4; np.rows = T; np.out = a->e8;

@@ -410,33 +410,15 @@ def fc_head_train(x, exp_x, w, exp_w, target, seed, layer_stream, *, dropout=Tru
 
 
 # ------------------------------------------------------------------ a vocabulary of classes
-def _vocab_work(x, w, index, train):
+def _vocab(train, x, w, index, *args):
+    """The native call; `args` are its arguments behind the layer's two tensors and two exponents."""
     def work(r):
         (T, F), V = x.shape, w.shape[0]
         return (6 if train else 2) * T * V * F, T * F * (2 if train else 1) + V * F * (5 if train else 1) + 8 * index.numel() + 4 * T
-    return work
-
-
-def _vocab_no_tokens(x, exp_w, w, temperature_log2, g32):
-    """What a call without tokens returns: the same shapes, nothing to learn."""
-    g32 = torch.zeros(w.shape, dtype=torch.int32, device=w.device) if g32 is None else g32.zero_()
-    return (torch.empty(0, dtype=torch.float32, device=x.device), torch.empty_like(x), exp_w.reshape(()) + (temperature_log2 - 7), g32,
-            torch.zeros(1, dtype=torch.int32, device=x.device))
-
-
-def _vocab_call(layer, index, ignore_index, top, exp_top, temperature_log2, train):
-    x, exp_x, w, exp_w = layer
-    if x.dim() == 2 and x.shape[0] == 0:
-        _need_cuda(x, exp_x, w, exp_w, index)
-        r = _vocab_no_tokens(x, exp_w, w, temperature_log2, train[-1] if train else None)
-        return r if train else r[0]
-    # at most: operands in copies, statistics, wanted logits, row sums; words cleared, maximum, copy and narrowing of the error; per
-    # piece of errors the product again, the wanted errors, two products and a copy
-    launches = 5
-    if train:
-        launches += 5 + 5 * vocab_pieces(x.shape[0], w.shape[0])
-    return _run("niti_vocab_loss_i8", launches, _vocab_work(x, w, index, bool(train)), native.vocab_loss, x, exp_x, w, exp_w, index,
-                ignore_index, top, exp_top, temperature_log2, bool(train), *train)
+    # at most: operands in copies, statistics, wanted logits, row sums; the error's maximum and its narrowing; per piece of errors the
+    # product again, the wanted errors and the two products that lead back
+    launches = 5 if not train else 7 + 3 * vocab_pieces(max(1, x.size(0)), max(1, w.size(0)))
+    return _run("niti_vocab_loss_i8", launches, work, native.vocab_loss, *args)
 
 
 def vocab_pieces(tokens, classes):
@@ -449,7 +431,7 @@ def vocab_loss(x, exp_x, w, exp_w, target, ignore_index=-100):
     """Softmax cross entropy of a last layer with a vocabulary of classes, without its logits: x int8 [tokens, features] and
     w int8 [classes, features] with their exponents, target int64 [tokens] -> float32 [tokens], -ln p of each token's class.
     Rows whose target is ignore_index: 0.  Other targets outside the vocabulary: NaN."""
-    return _vocab_call((x, exp_x, w, exp_w), target, ignore_index, None, None, 0, ())
+    return _vocab(False, x, w, target, x, exp_x, w, exp_w, target, ignore_index, None, None, 0, False)
 
 
 def vocab_train(x, exp_x, w, exp_w, target, ignore_index=-100, *, bits=7, loss_mode=ROUND_PSEUDO_STOCHASTIC, err_mode=ROUND_NEAREST,
@@ -460,8 +442,8 @@ def vocab_train(x, exp_x, w, exp_w, target, ignore_index=-100, *, bits=7, loss_m
     (units of 2^-7; rounding to nearest drops every probability below 2^-8, pseudo-stochastic below 2^-19), err_mode the error of
     x.  Stochastic modes draw from the seed's streams loss_stream (round_up(classes, 4) words a token) and err_stream.  Rows
     without a loss have no error."""
-    return _vocab_call((x, exp_x, w, exp_w), target, ignore_index, None, None, 0,
-                       (bits, loss_mode, err_mode, seed, loss_stream, err_stream, sample_offset, g32))
+    return _vocab(True, x, w, target, x, exp_x, w, exp_w, target, ignore_index, None, None, 0, True, bits, loss_mode, err_mode, seed,
+                  loss_stream, err_stream, sample_offset, g32)
 
 
 def vocab_distill_loss(x, exp_x, w, exp_w, index, top, exp_top, temperature_log2=0):
@@ -469,15 +451,15 @@ def vocab_distill_loss(x, exp_x, w, exp_w, index, top, exp_top, temperature_log2
     negative: no entry), top (int8 or int32, same shape) with exp_top those logits.  float32 [tokens],
     4^temperature_log2 * sum_k q_k (ln q_k - ln p[index_k]), q the softmax over the row's entries and p the student's over the
     vocabulary, both at temperature 2^temperature_log2.  Rows without an entry: 0.  Rows with a class outside the vocabulary: NaN."""
-    return _vocab_call((x, exp_x, w, exp_w), index, -1, top, exp_top, temperature_log2, ())
+    return _vocab(False, x, w, index, x, exp_x, w, exp_w, index, -1, top, exp_top, temperature_log2, False)
 
 
 def vocab_distill_train(x, exp_x, w, exp_w, index, top, exp_top, temperature_log2=0, *, bits=7, loss_mode=ROUND_PSEUDO_STOCHASTIC,
                         err_mode=ROUND_NEAREST, seed=None, loss_stream=0xFFFF, err_stream=1, sample_offset=0, g32=None):
     """vocab_distill_loss and the gradients of the sum of its losses, as vocab_train returns them (g32 in units of
     2^(exp_x - 7 + temperature_log2))."""
-    return _vocab_call((x, exp_x, w, exp_w), index, -1, top, exp_top, temperature_log2,
-                       (bits, loss_mode, err_mode, seed, loss_stream, err_stream, sample_offset, g32))
+    return _vocab(True, x, w, index, x, exp_x, w, exp_w, index, -1, top, exp_top, temperature_log2, True, bits, loss_mode, err_mode, seed,
+                  loss_stream, err_stream, sample_offset, g32)
 
 
 def update(w, g32, maxabs, mu, mode=ROUND_PSEUDO_STOCHASTIC, seed=None, rng_stream=0):
