@@ -488,6 +488,7 @@ struct ThinParams {
     const int32_t* exp_x; const int32_t* exp_w; int temperature;
     int32_t* piece_max; uint32_t* piece_sum;
     const long long* index; int32_t* logit;
+    int32_t* all_logits;                      // training: [rows][classes]; null: they are not kept
 };
 template <int T, bool ALIGNED>
 __global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinParams p) {
@@ -568,6 +569,11 @@ __global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinPara
         if (warp < p.rows) {  // a warp to each token: the piece's statistics, and the wanted classes in it
             const int lim = p.classes - piece * PIECE;
             const int32_t a = lane < lim ? s_logit[warp][lane] : INT_MIN, b = lane + 32 < lim ? s_logit[warp][lane + 32] : INT_MIN;
+            if (p.all_logits != nullptr) {
+                int32_t* to = p.all_logits + static_cast<long long>(warp) * p.classes + static_cast<long long>(piece) * PIECE;
+                if (lane < lim) to[lane] = a;
+                if (lane + 32 < lim) to[lane + 32] = b;
+            }
             const int32_t m = __reduce_max_sync(0xFFFFFFFFu, max(a, b));
             unsigned long long e = 0;
             if (lane < lim) e = exp_weight(static_cast<unsigned>(m) - static_cast<unsigned>(a), sc);
@@ -826,6 +832,144 @@ __global__ void __launch_bounds__(256) vocab_patch_kernel(const int* entries, lo
     if ((w & (1 << 23)) && j >= 0 && j < count) err[(i % rows) * pitch + j] = static_cast<int8_t>(w >> 24);
 }
 
+// ---------------------------------------------------------------------------------------------- a few tokens' way back
+// Both products that lead back for the tokens of vocab_thin_kernel, from the logits it kept (no more bytes than a sixteenth of w's
+// features): w read once, the gradient written once, which is nearly all there is to do (an outer product of a few rows).  A thread
+// owns four features and walks the classes, four at a time: their errors with the features' tokens (dp4a over tokens) are the
+// gradient, which leaves at once; with w (dp4a over classes) they add up to the features' error, which is added to e32 at the
+// end.  2 x 1024 x 100000: 99 us, 5.2 TB/s; the tiles of umma_gemm_two, which are all epilogue here, 119 behind the 36 of
+// vocab_kernel (from five tokens on they are ahead: 8 x 1024 x 100000 with 16 tokens' room 161).
+constexpr int BACK_THREADS = 256, BACK_ROWS = 64, BACK_FEATURES = 4 * BACK_THREADS;
+struct BackParams {
+    const int32_t* logits;                    // [T][V]
+    const int8_t* x; const int8_t* w;         // rows of F bytes
+    int T, F, V, F4;
+    int32_t* e32; int32_t* g32; unsigned* g_max;
+    const int32_t* exp_x; const int32_t* exp_w; int temperature;
+    const int4* row_stat; const int* entries; int num_entries;
+    int mode; const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
+};
+// One class's error from its logit: what vocab_kernel computes, a value at a time.
+__device__ int8_t error_of(int32_t a, const int4& stat, const ExpScale& sc, const BackParams& p, int t, int v) {
+    if ((stat.w & (1 << 23)) && (stat.w & 0x3FFFF) == v) return static_cast<int8_t>(stat.w >> 24);
+    for (int k = 0; k < p.num_entries; ++k) {
+        const int w = __ldg(p.entries + k * p.T + t);
+        if ((w & (1 << 23)) && (w & 0x3FFFF) == v) return static_cast<int8_t>(w >> 24);
+    }
+    const uint32_t E = exp_weight(static_cast<unsigned>(stat.x) - static_cast<unsigned>(a), sc);
+    const int32_t y = static_cast<int32_t>(mul_hi(E, static_cast<uint32_t>(stat.y)) >> stat.z);
+    uint32_t rnd = 0;
+    if (p.mode == ROUND_STOCHASTIC) rnd = random_word(*p.seed, p.rng_stream, (p.rng_offset + t) * static_cast<unsigned long long>((p.V + 3) / 4 * 4) + v);
+    return narrow(y, 23, p.mode, rnd);
+}
+// VEC: features side by side that a thread loads and stores at once (4, or 2 or 1 where rows are no multiples of four)
+template <int NT, int VEC>
+__global__ void __launch_bounds__(BACK_THREADS) vocab_back_thin_kernel(const BackParams p) {
+    constexpr int TQ = (NT + 3) / 4;
+    __shared__ uint32_t s_tokens[BACK_ROWS][TQ];          // a class's errors, four tokens to a word
+    __shared__ uint32_t s_classes[BACK_ROWS / 4][TQ * 4]; // a token's errors, four classes to a word
+    __shared__ unsigned s_max[BACK_THREADS / 32];
+    const int tid = threadIdx.x, f0 = static_cast<int>(blockIdx.y) * BACK_FEATURES;
+    const ExpScale sc = exp_scale(*p.exp_x + *p.exp_w - p.temperature);
+    int f[4];
+    uint32_t xq[TQ][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[j] = f0 + j / VEC * (VEC * BACK_THREADS) + VEC * tid + j % VEC;
+#pragma unroll
+        for (int q = 0; q < TQ; ++q) {
+            xq[q][j] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (4 * q + k < p.T && f[j] < p.F) xq[q][j] |= static_cast<uint32_t>(static_cast<uint8_t>(p.x[static_cast<long long>(4 * q + k) * p.F + f[j]])) << (8 * k);
+        }
+    }
+    int acc[NT][4], hi = 0, lo = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[t][j] = 0;
+    const int batches = (p.V + BACK_ROWS - 1) / BACK_ROWS;
+    for (int batch = blockIdx.x; batch < batches; batch += gridDim.x) {
+        const int v0 = batch * BACK_ROWS;
+        __syncthreads();
+        for (int i = tid; i < TQ * 4 * BACK_ROWS; i += BACK_THREADS) {
+            const int t = i / BACK_ROWS, r = i % BACK_ROWS, v = v0 + r;
+            int8_t e = 0;
+            if (t < p.T && v < p.V) e = error_of(__ldg(p.logits + static_cast<long long>(t) * p.V + v), __ldg(p.row_stat + t), sc, p, t, v);
+            reinterpret_cast<int8_t*>(s_tokens)[r * TQ * 4 + t] = e;
+            reinterpret_cast<int8_t*>(s_classes)[(r >> 2) * TQ * 16 + t * 4 + (r & 3)] = e;
+        }
+        __syncthreads();
+        if (f[0] >= p.F) continue;
+#pragma unroll 2
+        for (int rq = 0; rq < BACK_ROWS / 4; ++rq) {
+            const int v = v0 + 4 * rq;
+            if (v >= p.V) break;
+            uint32_t row[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                row[k] = 0;
+                if (v + k < p.V) {
+                    const int8_t* at = p.w + static_cast<long long>(v + k) * p.F;
+#pragma unroll
+                    for (int j = 0; j < 4; j += VEC)
+                        if (f[j] < p.F) {
+                            if (VEC == 4) row[k] = __ldg(reinterpret_cast<const uint32_t*>(at + f[j]));
+                            else if (VEC == 2) row[k] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(at + f[j]))) << (8 * j);
+                            else row[k] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(at + f[j]))) << (8 * j);
+                        }
+                }
+            }
+            // four classes of a feature to a word
+            const uint32_t a = __byte_perm(row[0], row[1], 0x5140), b = __byte_perm(row[2], row[3], 0x5140);
+            const uint32_t c = __byte_perm(row[0], row[1], 0x7362), d = __byte_perm(row[2], row[3], 0x7362);
+            const uint32_t col[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x5410), __byte_perm(c, d, 0x7632)};
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int e = static_cast<int>(s_classes[rq][t]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[t][j] = __dp4a(static_cast<int>(col[j]), e, acc[t][j]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (v + k >= p.V) break;
+                int g[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int q = 0; q < TQ; ++q) {
+                    const int e = static_cast<int>(s_tokens[4 * rq + k][q]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g[j] = __dp4a(static_cast<int>(xq[q][j]), e, g[j]);
+                }
+                hi = __vimax3_s32(__vimax3_s32(hi, g[0], g[1]), g[2], g[3]);
+                lo = __vimin3_s32(__vimin3_s32(lo, g[0], g[1]), g[2], g[3]);
+                int32_t* to = p.g32 + static_cast<long long>(v + k) * p.F;
+#pragma unroll
+                for (int j = 0; j < 4; j += VEC)
+                    if (f[j] < p.F) {
+                        if (VEC == 4) *reinterpret_cast<int4*>(to + f[j]) = make_int4(g[0], g[1], g[2], g[3]);
+                        else if (VEC == 2) *reinterpret_cast<int2*>(to + f[j]) = make_int2(g[j], g[j + 1]);
+                        else to[f[j]] = g[j];
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (t < p.T && f[j] < p.F && acc[t][j] != 0) atomicAdd(p.e32 + static_cast<long long>(t) * p.F4 + f[j], acc[t][j]);
+    const unsigned m = __reduce_max_sync(0xFFFFFFFFu, max(static_cast<unsigned>(hi), static_cast<unsigned>(-lo)));
+    if ((tid & 31) == 0) s_max[tid >> 5] = m;
+    __syncthreads();
+    if (tid == 0) {
+        unsigned x = 0;
+#pragma unroll
+        for (int w = 0; w < BACK_THREADS / 32; ++w) x = max(x, s_max[w]);
+        if (x != 0) atomicMax(p.g_max, x);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- the error's narrowing
 struct NarrowParams {
     const int32_t* e32; int F, F4, rows;      // [rows][F4], F of them written
@@ -908,6 +1052,19 @@ __global__ void __launch_bounds__(256) vocab_narrow_kernel(const NarrowParams p)
 }
 
 // ---------------------------------------------------------------------------------------------- host side
+template <int NT>
+int launch_back_inst(const BackParams& p, cudaStream_t st) {
+    const int y = (p.F + BACK_FEATURES - 1) / BACK_FEATURES, batches = (p.V + BACK_ROWS - 1) / BACK_ROWS, most = (3 * sm_count() + y - 1) / y;
+    const dim3 grid(static_cast<unsigned>(batches < most ? batches : most), static_cast<unsigned>(y));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.w);
+    if (p.F % 4 == 0 && at % 4 == 0)      vocab_back_thin_kernel<NT, 4><<<grid, BACK_THREADS, 0, st>>>(p);
+    else if (p.F % 2 == 0 && at % 2 == 0) vocab_back_thin_kernel<NT, 2><<<grid, BACK_THREADS, 0, st>>>(p);
+    else                                  vocab_back_thin_kernel<NT, 1><<<grid, BACK_THREADS, 0, st>>>(p);
+    return launched(cudaGetLastError());
+}
+int launch_back(const BackParams& p, cudaStream_t st) {
+    return p.T == 1 ? launch_back_inst<1>(p, st) : p.T == 2 ? launch_back_inst<2>(p, st) : launch_back_inst<THIN_TOKENS>(p, st);
+}
 // err_calc of the whole error; `summed`: its maximum is still to be found
 int narrow_error(NarrowParams p, bool summed, cudaStream_t st) {
     const long long words = static_cast<long long>(p.rows) * (p.F4 / 4), blocks = (words + 1023) / 1024, most = 4ll * sm_count();
@@ -1026,7 +1183,7 @@ int launch_thin(int T, const ThinParams& p, size_t smem, cudaStream_t st) {
 // The workspace of a call.
 struct VocabPlan {
     int pieces, pitch, piece;   // row pitch of the operands; classes whose errors are in the workspace at a time
-    size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, bytes;
+    size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, logits_at, bytes;
 };
 // Errors in the workspace at a time.  Pieces of 37 column tiles: 148 SMs are 74 pairs of thread blocks, so the errors' tiles and the weight
 // gradient's come in whole waves where the tokens, or the features, fill an even number of 256-row tiles.
@@ -1050,11 +1207,13 @@ VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     p.sum_at = take(4 * t * p.pieces);
     p.logit_at = take(4 * t * k);
     p.word_at = take(16);
-    if (p.pitch != F && (train || !thin_serves(T, F))) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
+    const bool thin = thin_serves(T, F);
+    if (p.pitch != F && !thin) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
     if (train) {
         p.stat_at = take(16 * t);
         p.entry_at = take(4 * t * k);
-        p.err_at = take(t * p.piece);
+        if (thin) p.logits_at = take(4 * t * V);
+        else p.err_at = take(t * p.piece);
         p.e32_at = take(4 * t * up(F, 4));
     }
     p.bytes = at;
@@ -1100,7 +1259,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     // operands whose rows are no multiples of 16 bytes go through copies that are
     const int8_t *x = a->x, *w = a->w;
     const bool thin = thin_serves(T, F);
-    if (pl.pitch != F && (train || !thin)) {
+    if (pl.pitch != F && !thin) {
         x = reinterpret_cast<int8_t*>(ws + pl.x_at);
         w = reinterpret_cast<int8_t*>(ws + pl.w_at);
         if (int e = align_rows(a->x, T, ws + pl.x_at, a->w, V, ws + pl.w_at, F, pl.pitch, st)) return e;
@@ -1117,7 +1276,8 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     const long long wanted = static_cast<long long>(T) * K;
     if (thin) {
         ThinParams tp{};
-        tp.x = x; tp.w = w; tp.x_pitch = tp.pitch = w == a->w ? F : pl.pitch;
+        tp.x = x; tp.w = w; tp.x_pitch = tp.pitch = F;
+        if (train) tp.all_logits = reinterpret_cast<int32_t*>(ws + pl.logits_at);
         tp.F = F; tp.rows = T; tp.classes = V; tp.pieces = pl.pieces; tp.entries = K;
         tp.exp_x = a->exp_x; tp.exp_w = a->exp_w; tp.temperature = a->temperature_log2;
         tp.piece_max = vp.piece_max; tp.piece_sum = vp.piece_sum; tp.index = index; tp.logit = logit;
@@ -1155,13 +1315,13 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         return plan;
     };
     GemmTwoPlan plan{};
-    if (train) plan = piece_calls(0, pl.piece < V ? pl.piece : V);
-    const bool summed = train && (plan.splits > 1 || pl.piece < V);  // e32 comes in several parts
+    if (train && !thin) plan = piece_calls(0, pl.piece < V ? pl.piece : V);
+    const bool summed = train && (thin || plan.splits > 1 || pl.piece < V);  // e32 comes in several parts
     if (train) {
         fp.row_stat = reinterpret_cast<int4*>(ws + pl.stat_at);
         fp.entry_err = reinterpret_cast<int*>(ws + pl.entry_at);
         fp.err_exp = words; fp.clear[0] = reinterpret_cast<uint32_t*>(words + 1); fp.clear[1] = reinterpret_cast<uint32_t*>(words + 2); fp.clear[2] = a->grad_maxabs;
-        if (plan.splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
+        if (thin || plan.splits > 1) { fp.zero = reinterpret_cast<uint4*>(ws + pl.e32_at); fp.zero_count = static_cast<long long>(T) * F4 / 4; }
         fp.round_mode = a->loss_round;
         fp.seed = reinterpret_cast<const unsigned long long*>(a->seed); fp.rng_stream = a->loss_stream; fp.rng_offset = a->sample_offset;
     }
@@ -1178,7 +1338,18 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     const bool patch = a->top != nullptr && static_cast<long long>(T) * pl.piece * K > (1ll << 30);
     if (a->top != nullptr && !patch) { vp.entries = fp.entry_err; vp.num_entries = K; }
     vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
-    for (int v0 = 0; v0 < V; v0 += pl.piece) {
+    if (thin) {
+        BackParams bp{};
+        bp.logits = reinterpret_cast<const int32_t*>(ws + pl.logits_at);
+        bp.x = x; bp.w = w; bp.T = T; bp.F = F; bp.V = V; bp.F4 = F4;
+        bp.e32 = e32; bp.g32 = a->g32; bp.g_max = a->grad_maxabs;
+        bp.exp_x = a->exp_x; bp.exp_w = a->exp_w; bp.temperature = a->temperature_log2;
+        bp.row_stat = fp.row_stat; bp.mode = a->loss_round;
+        if (a->top != nullptr) { bp.entries = fp.entry_err; bp.num_entries = K; }
+        bp.seed = fp.seed; bp.rng_stream = a->loss_stream; bp.rng_offset = a->sample_offset;
+        if (int e = launch_back(bp, st)) return e;
+    }
+    for (int v0 = 0; v0 < V && !thin; v0 += pl.piece) {
         const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
         vp.first = v0;
         if (int e = run_vocab(a->loss_round, x, w, T, F, pl.pitch, count, &vp, a->status, st)) return e;
