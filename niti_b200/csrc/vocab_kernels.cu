@@ -129,7 +129,7 @@ __device__ __forceinline__ void vocab_load(uint8_t* smem, uint64_t* full_bar, ui
     const uint32_t rank = TWO ? __shfl_sync(0xFFFFFFFFu, cluster_ctarank(), 0) : 0u;
     const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
     const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar);
-    const uint32_t block_tx = static_cast<uint32_t>((TWO ? 2 : 1) * (PANEL_BYTES + Cfg::B_PANEL_BYTES));
+    const uint32_t block_tx = static_cast<uint32_t>(keep_reg((TWO ? 2 : 1) * (p.a_bytes + Cfg::B_PANEL_BYTES)));
     uint32_t s = 0, ph = 1;
     for (int tile = first; tile < total; tile += step) {
         int m_pair, n_t;
@@ -1135,7 +1135,9 @@ int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitc
     const bool pair = tile.pair;
     CUtensorMap ma, mb;
     uint64_t dims[2] = {static_cast<uint64_t>(F), static_cast<uint64_t>(T)}, str[1] = {static_cast<uint64_t>(pitch)};
-    uint32_t box[2] = {128, 128};
+    // a single row tile's box is no higher than its tokens (in eights): what the MMAs read of the other rows ends in rows nobody looks at
+    const int a_rows = m128 == 1 ? (T + 7) / 8 * 8 : BLOCK_M;
+    uint32_t box[2] = {128, static_cast<uint32_t>(a_rows)};
     if (int e = encode_map(&ma, x, false, 2, dims, str, box)) return e;
     dims[1] = count; box[1] = pair ? VBN / 2 : bn;
     if (int e = encode_map(&mb, w + static_cast<long long>(p->first) * pitch, false, 2, dims, str, box)) return e;
@@ -1143,7 +1145,7 @@ int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitc
     g = GemmParams{};
     g.M = T; g.N = count; g.K = F; g.num_kb = (F + 127) / 128; g.splits = 1;
     g.m_tiles = pair ? (m128 + 1) / 2 : m128; g.n_tiles = (count + bn - 1) / bn;
-    g.status = status;
+    g.a_bytes = a_rows * ROW_BYTES; g.status = status;
     g.group_m = (static_cast<long long>(T) + count) * F > (48ll << 20) ? 8 : 0;  // as umma_gemm orders its tiles
     g.fd_mn = make_fastdiv(g.m_tiles * g.n_tiles); g.fd_n = make_fastdiv(g.n_tiles); g.fd_tw = make_fastdiv(1); g.fd_th = make_fastdiv(1);
     if (pair) return launch_vocab<true, VBN>(what, ma, mb, *p, st);
