@@ -70,9 +70,11 @@ class Trainer:
         ti_torch.GLOBAL_MAX_GROUP = (group if group is not None else True) if self.global_exact else None
         if self.global_exact:
             self.use_graph = use_graph = False
-        # weight-gradient kernels run beside the error-backward kernels on a second stream (joined before the update)
-        self.side = torch.cuda.Stream(device=self.device) if (wgrad_side_stream and not keep_gradients) else None
         self.layers = model.weighted_layers()
+        # weight-gradient kernels run beside the error-backward kernels on a second stream (joined before the update, so there is
+        # none where no layer forks it: a captured step may not wait for a stream that it has not reached)
+        forks = any(isinstance(l, ti_torch.TiConv2d) and not l.first_layer for l in self.layers)
+        self.side = torch.cuda.Stream(device=self.device) if (wgrad_side_stream and not keep_gradients and forks) else None
         # With more than one rank the exchange is either ONE kernel per rank over peer memory (reduce-scatter of the
         # gradients, update of the own slice, new weights stored into every replica: ops.dp_update) when the ranks sit
         # on different GPUs of one node, or an NCCL all-reduce of the bucket followed by the update launch.
