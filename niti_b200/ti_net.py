@@ -7,7 +7,7 @@ from torch.nn.modules import Module
 
 from . import ops, ti_torch
 from .ti_loss import TiLoss
-from .ti_torch import RangeEstimate, TiDropout, TiFloatToInt8, TiLinear, exp_tensor
+from .ti_torch import RangeEstimate, TiDropout, TiFloatToInt8, TiLinear, TiVocabHead, exp_tensor
 
 
 class TiNet(Module):
@@ -49,6 +49,30 @@ class TiNet(Module):
             else:
                 x = layer.backward(x)
 
+    def vocab_head(self):
+        """The last layer if it is a TiVocabHead, else None."""
+        last = self.forward_layers[-1] if len(self.forward_layers) else None
+        return last if isinstance(last, TiVocabHead) else None
+
+    def _vocab_body(self, x):
+        h = TiFloatToInt8(x)
+        for l in list(self.forward_layers)[:-1]:
+            h = l(h)
+        return h
+
+    def losses(self, x, target):
+        """A TiVocabHead network's loss of every row, without training; ``target`` as in train_step."""
+        head, h = self.vocab_head(), self._vocab_body(x)
+        return head.distill_loss(h, target[:3], *target[3:]) if isinstance(target, tuple) else head.loss(h, target)
+
+    def _vocab_step(self, x, target):
+        head, h = self.vocab_head(), self._vocab_body(x)
+        loss, e = head.distill_step(h, target[:3], *target[3:]) if isinstance(target, tuple) else head.train_step(h, target)
+        self.out, self.out_exp = loss, e[1]
+        for l in reversed(list(self.forward_layers)[:-1]):
+            e = l.backward(e)
+        return loss
+
     def _fusable_head(self, batch):
         """(number of head layers, has dropout) if the network ends in [TiDropout,] TiLinear of a size the
         one-kernel classifier head takes, else None."""
@@ -65,7 +89,12 @@ class TiNet(Module):
     def train_step(self, x, target):
         """forward(x) followed by backward(target), with the same results; when the network ends in
         [TiDropout,] TiLinear the whole classifier head (dropout, FC forward, loss, FC backward, update)
-        runs as one kernel instead of eleven."""
+        runs as one kernel instead of eleven.
+
+        A network that ends in a TiVocabHead trains on that layer's losses instead, which it returns (float32, one to each
+        row); ``target`` may then be a teacher's top logits, (classes, logits, exponent[, temperature_log2])."""
+        if self.vocab_head() is not None:
+            return self._vocab_step(x, target)
         head = self._fusable_head(x.shape[0])
         if head is None:
             out = self.forward(x)

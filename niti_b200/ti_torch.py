@@ -232,6 +232,69 @@ class TiLinear(UpdateWeight):
         return err_out, err_exp
 
 
+class TiVocabHead(TiLinear):
+    """A last layer whose classes are a vocabulary: TiLinear, TiLoss and TiLinear.backward (:241-266, ti_loss.py:6-36) in one call
+    that never holds the logits, with a softmax of 30 bits (TiLoss has 11: 2048 equal classes have no error).  Rows are tokens; leading
+    dimensions (batch, position) are taken together.  No counterpart in the reference, whose networks end in 10 classes.
+
+    ``forward`` and ``backward`` are TiLinear's, for the few tokens whose logits are wanted.  Rows whose target is ``ignore_index``
+    have neither loss nor error; a target outside the vocabulary makes its row's loss NaN."""
+
+    def __init__(self, in_features, out_features, ignore_index=-100):
+        super(TiVocabHead, self).__init__(in_features, out_features, last_layer=True)
+        self.ignore_index = ignore_index
+
+    def _rows(self, input):
+        act, exp_in = input
+        dev = act.device
+        return act.reshape(-1, act.shape[-1]).contiguous(), exp_tensor(exp_in, dev), self.weight, exp_tensor(self.weight_exp, dev)
+
+    def _teacher(self, teacher, dev):
+        index, top, exp_top = teacher
+        return (index.to(device=dev, dtype=torch.int64).reshape(-1, index.shape[-1]).contiguous(),
+                top.to(device=dev).reshape(-1, top.shape[-1]).contiguous(), exp_tensor(exp_top, dev))
+
+    def _target(self, target, dev):
+        return target.to(device=dev, dtype=torch.int64).reshape(-1).contiguous()
+
+    def loss(self, input, target):
+        """(act int8 [..., in], exp), target [...] -> float32 [...]: -ln p of every token's class."""
+        layer = self._rows(input)
+        return ops.vocab_loss(*layer, self._target(target, layer[0].device), self.ignore_index).view(input[0].shape[:-1])
+
+    def distill_loss(self, input, teacher, temperature_log2=0):
+        """teacher = (classes int64 [..., k], their logits int8 or int32 [..., k], exponent): its k largest logits of every token,
+        negative classes for none -> float32 [...], see ops.vocab_distill_loss."""
+        layer = self._rows(input)
+        return ops.vocab_distill_loss(*layer, *self._teacher(teacher, layer[0].device), temperature_log2).view(input[0].shape[:-1])
+
+    def train_step(self, input, target):
+        """loss() with its backward pass: (float32 [...], (err int8 [..., in], exp)); updates the weights."""
+        return self._step(input, target, None, 0)
+
+    def distill_step(self, input, teacher, temperature_log2=0):
+        """distill_loss() with its backward pass, as train_step."""
+        return self._step(input, None, teacher, temperature_log2)
+
+    def _step(self, input, target, teacher, temperature_log2):
+        if GLOBAL_MAX_GROUP is not None:
+            raise RuntimeError("TiVocabHead: the global-exact data-parallel mode is not implemented")
+        layer = self._rows(input)
+        dev, shape = layer[0].device, input[0].shape
+        how = dict(bits=BITWIDTH, loss_mode=_mode(VOCAB_ROUND_METHOD), err_mode=_mode(ERROR_ROUND_METHOD), seed=RNG_SEED(dev), loss_stream=0xFFFF,
+                   err_stream=16 * self.layer_id + 1, sample_offset=SAMPLE_OFFSET * (layer[0].shape[0] // shape[0] if shape[0] else 1), g32=self.grad_buffer)
+        if teacher is None:
+            loss, err, err_exp, g32, g_max = ops.vocab_train(*layer, self._target(target, dev), self.ignore_index, **how)
+        else:
+            loss, err, err_exp, g32, g_max = ops.vocab_distill_train(*layer, *self._teacher(teacher, dev), temperature_log2, **how)
+        self.__dict__.update(act_in=input, act_in_exp=input[1], err_exp=err_exp, grad_int32acc=g32, grad_maxabs=g_max)
+        if self.grad_ready is not None:
+            self.grad_ready(self)
+        if not self.defer_update:
+            self.weight_update()
+        return loss.view(shape[:-1]), (err.view(shape), err_exp)
+
+
 class TiReLU(Module):
     """Integer ReLU (:268-290).  ``fused=True`` marks a ReLU whose forward was already applied by
     the preceding convolution's requantisation; backward is the same either way because
@@ -530,6 +593,9 @@ ACT_ROUND_METHOD = RoundShift
 ERROR_ROUND_METHOD = RoundShift
 
 GRAD_ROUND_METHOD = PstoShift
+# Errors of a vocabulary's logits, which are mostly far below half of int8's unit of 2^-7: RoundShift would drop all of them below
+# 2^-8, PstoShift those below 2^-19, StoShift none (at 20 instructions of random words a logit).
+VOCAB_ROUND_METHOD = PstoShift
 WEIGHT_INIT_METHOD = UniformWeights
 
 FUSE_REQUANT = True    # convolutions narrow to int8 inside their own kernel (predicted shift, verified, redone if wrong)

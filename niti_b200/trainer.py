@@ -105,14 +105,17 @@ class Trainer:
         # one-CTA-per-SM contraction kernels and delay the cooperative ones, which need every SM free).
         self.x = torch.zeros((local_batch,) + tuple(in_shape), dtype=torch.float32, device=self.device)
         self.t = torch.zeros((local_batch,), dtype=torch.int64, device=self.device)
-        # two result slots, used alternately: step i's logits stay readable while step i+1 writes the other slot
-        self._out_hosts = [torch.zeros((local_batch, self.layers[-1].weight.shape[0]), dtype=torch.int8).pin_memory() for _ in range(2)]
+        # two result slots, used alternately: step i's logits stay readable while step i+1 writes the other slot.  A network that
+        # ends in a TiVocabHead hands back its rows' losses, and beside them the exponent of the error that it trained on.
+        vocab = model.vocab_head() is not None
+        out_shape, out_type = ((local_batch,), torch.float32) if vocab else ((local_batch, self.layers[-1].weight.shape[0]), torch.int8)
+        self._out_hosts = [torch.zeros(out_shape, dtype=out_type).pin_memory() for _ in range(2)]
         self._exp_hosts = [torch.zeros((), dtype=torch.int32).pin_memory() for _ in range(2)]
         self._done = [torch.cuda.Event() for _ in range(2)]
         self._res_slot = 0
         self.out_host, self.exp_host = self._out_hosts[0], self._exp_hosts[0]
         self.h2d_bytes = self.x.numel() * 4 + self.t.numel() * 8
-        self.d2h_bytes = self.out_host.numel() + 4
+        self.d2h_bytes = self.out_host.numel() * self.out_host.element_size() + 4
         ti_torch.set_seed(seed, self.device)
         self.sample_offset = rank * local_batch if sample_offset is None else int(sample_offset)
         ti_torch.SAMPLE_OFFSET = self.sample_offset
@@ -330,9 +333,9 @@ class Trainer:
         self._pf_key = (x_host.data_ptr(), target_host.data_ptr(), slot)
 
     def step(self, x_host, target_host, prefetch_next=None):
-        """x_host float32 [B,3,32,32] and target_host int64 [B] in (pinned) host memory.
-        Returns (pinned int8 logits [B, classes], pinned int32 exponent); valid after the
-        stream is synchronised (``Trainer.sync``).  ``prefetch_next=(x, t)``: the next batch, whose copy
+        """x_host float32 [B,3,32,32] (in_shape) and target_host int64 [B] in (pinned) host memory.
+        Returns (pinned int8 logits [B, classes], pinned int32 exponent) (of a network that ends in a TiVocabHead: float32
+        losses [B]); valid after the stream is synchronised (``Trainer.sync``).  ``prefetch_next=(x, t)``: the next batch, whose copy
         then runs beside this step's kernels."""
         if self._failed is not None:
             raise RuntimeError(f"{self._failed}; the trainer takes no further steps until reset_exchange()")

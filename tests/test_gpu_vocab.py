@@ -266,3 +266,116 @@ def test_refusals():
         with pytest.raises((RuntimeError, TypeError)):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+# ----------------------------------------------------------------------------- the layer, the network, the trainer
+def mlp(widths, vocab, seed):
+    """A network of linear layers that ends in a vocabulary, and its weights on the host."""
+    from torch.nn import Sequential
+    from niti_b200 import ti_torch
+    from niti_b200.ti_net import TiNet
+    rng = np.random.default_rng(seed)
+    net = TiNet()
+    layers = []
+    for a, b in zip(widths, widths[1:]):
+        layers += [ti_torch.TiLinear(a, b), ti_torch.TiReLU()]
+    layers += [ti_torch.TiVocabHead(widths[-1], vocab)]
+    net.forward_layers = Sequential(*layers)
+    net.assign_layer_ids()
+    host = []
+    for l in net.weighted_layers():
+        w = np.clip(np.rint(rng.standard_normal(tuple(l.weight.shape)) * 30), -127, 127).astype(np.int8)
+        e = -9 - int(np.log2(w.shape[1]) / 2)
+        l.weight, l.weight_exp = cu(w), ti_torch.exp_tensor(e, DEV)
+        host.append([w, e])
+    return net, host
+
+
+def oracle_step(host, x, target=None, teacher=None, temperature_log2=0, mu=5):
+    """One step of that network; updates `host` in place and returns the losses."""
+    a, e = O.float_to_int8(x)
+    acts = []
+    for w, we in host[:-1]:
+        acts.append((a, e))
+        a, e, _ = O.act_calc(O.int8_mm(a, w.T), e + we)
+        acts.append((a, e))
+        a = np.maximum(a, 0).astype(np.int8)
+    w, we = host[-1]
+    kw = dict(top=teacher[1], exp_top=teacher[2], temperature_log2=temperature_log2) if teacher else {}
+    r = VO.vocab(a, e, w, we, teacher[0] if teacher else target, err_stream=16 * (len(host) - 1) + 1, **kw)
+    err, err_e = r["e8"], r["exp_err"]
+    grads = [r["g32"]]
+    for i in range(len(host) - 2, -1, -1):
+        pre, inp = acts[2 * i + 1][0], acts[2 * i][0]
+        err = np.where(pre > 0, err, 0).astype(np.int8)
+        grads.insert(0, O.int8_mm(err.T, inp))
+        if i > 0:
+            err, _ = O.err_calc(O.int8_mm(err, host[i][0]))
+    for i, g in enumerate(grads):
+        host[i][0] = O.weight_update(host[i][0], g, mu)[0]
+    return r["loss"]
+
+
+def test_a_network_learns_tokens_and_then_from_a_teacher():
+    from niti_b200 import ti_torch
+    ti_torch.GRAD_BITWIDTH, ti_torch.TRAINING = 5, True
+    T, V, K = 130, 700, 7
+    net, host = mlp([24, 48, 64], V, 3)
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((T, 24)).astype(np.float32)
+    y = rng.integers(0, V, T)
+    y[::9] = -100
+    for _ in range(3):
+        before = net.losses(cu(x), cu(y))
+        loss = net.train_step(cu(x), cu(y))
+        assert torch.equal(before, loss)
+        same_loss(loss, oracle_step(host, x, y))
+    teacher = (np.stack([rng.choice(V, K, replace=False) for _ in range(T)]), rng.integers(-100, 101, (T, K)).astype(np.int8), -4)
+    teacher[0][5, 2:] = -1
+    on_gpu = (cu(teacher[0]), cu(teacher[1]), teacher[2], 1)
+    for _ in range(2):
+        before = net.losses(cu(x), on_gpu)
+        loss = net.train_step(cu(x), on_gpu)
+        assert torch.equal(before, loss)
+        same_loss(loss, oracle_step(host, x, teacher=teacher, temperature_log2=1))
+    for l, (w, _) in zip(net.weighted_layers(), host):
+        same(l.weight, w, "weights")
+    ops.check_status(DEV)
+
+
+def test_tokens_in_batches_of_positions():
+    from niti_b200 import ti_torch
+    net, _ = mlp([32], 300, 6)
+    head = net.vocab_head()
+    rng = np.random.default_rng(7)
+    x = cu(rng.integers(-100, 101, (5, 9, 32)).astype(np.int8))
+    y = cu(rng.integers(0, 300, (5, 9)))
+    e = ti_torch.exp_tensor(-7, DEV)
+    head.defer_update = True
+    loss, (err, err_exp) = head.train_step((x, e), y)
+    assert loss.shape == (5, 9) and err.shape == x.shape
+    flat, (err1, err_exp1) = head.train_step((x.view(45, 32), e), y.view(45))
+    assert torch.equal(loss.view(-1), flat) and torch.equal(err.view(45, 32), err1) and int(err_exp) == int(err_exp1)
+    assert torch.equal(head.loss((x, e), y), loss)
+    first = head.loss((x.transpose(0, 1), e), y.t())  # positions first, not contiguous
+    assert torch.equal(first, loss.t())
+
+
+def test_trainer_replays_steps_of_a_vocabulary():
+    from niti_b200 import ti_torch
+    from niti_b200.trainer import Trainer
+    ti_torch.GRAD_BITWIDTH, ti_torch.TRAINING = 5, True
+    T, V = 64, 500
+    net, host = mlp([40, 32], V, 11)
+    rng = np.random.default_rng(12)
+    tr = Trainer(net, T, DEV, in_shape=(40,), warmup_steps=1, seed=1)
+    for _ in range(4):  # one eager step, then replays
+        x, y = rng.standard_normal((T, 40)).astype(np.float32), rng.integers(0, V, T)
+        r = tr.step(torch.from_numpy(x).pin_memory(), torch.from_numpy(y).pin_memory())
+        out, _ = r.wait()
+        want = oracle_step(host, x, y)
+        got = out.numpy().astype(np.float64)
+        assert np.all(np.abs(got - want) <= np.abs(want) * 2.0 ** -24 + 1e-11)
+    for l, (w, _) in zip(net.weighted_layers(), host):
+        same(l.weight, w, "weights")
+    ti_torch.SAMPLE_OFFSET = 0
