@@ -51,8 +51,8 @@ class TiNet(Module):
 
     def vocab_head(self):
         """The last layer if it is a TiVocabHead, else None."""
-        last = self.forward_layers[-1] if len(self.forward_layers) else None
-        return last if isinstance(last, TiVocabHead) else None
+        last = list(self.forward_layers)[-1:]
+        return last[0] if last and isinstance(last[0], TiVocabHead) else None
 
     def _vocab_body(self, x):
         h = TiFloatToInt8(x)

@@ -107,7 +107,8 @@ class Trainer:
         self.t = torch.zeros((local_batch,), dtype=torch.int64, device=self.device)
         # two result slots, used alternately: step i's logits stay readable while step i+1 writes the other slot.  A network that
         # ends in a TiVocabHead hands back its rows' losses, and beside them the exponent of the error that it trained on.
-        vocab = model.vocab_head() is not None
+        head = getattr(model, "vocab_head", None)
+        vocab = head is not None and head() is not None
         out_shape, out_type = ((local_batch,), torch.float32) if vocab else ((local_batch, self.layers[-1].weight.shape[0]), torch.int8)
         self._out_hosts = [torch.zeros(out_shape, dtype=out_type).pin_memory() for _ in range(2)]
         self._exp_hosts = [torch.zeros((), dtype=torch.int32).pin_memory() for _ in range(2)]
