@@ -209,6 +209,13 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
                  ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
+// ----------------------------------------------------------------------------- dependent launches
+// Of a kernel launched with programmatic stream serialisation: everything the kernel before it has written is there behind dependents_wait
+// (which EVERY thread block executes: a block that left without it could let the kernel behind this one overtake the one before);
+// dependents_start lets the kernel behind this one begin with what comes in front of its own wait.
+__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ----------------------------------------------------------------------------- tensor memory
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");

@@ -390,7 +390,8 @@ __device__ __forceinline__ void store_piece(int8_t* at, int cols, const uint32_t
 // Plain products: int32 out (+ max|acc|).  cta_first, cta_step: the tiles of this thread block (of a pair of them)
 // PLAIN: a result whose rows are no whole 16-byte groups (p.plain_out) leaves the staging tiles by ordinary stores, a row's 64 columns
 // to a warp at a time (918 x 1426, 40001 classes: 113 us; through a padded copy 113 + 147).
-template <int BN, bool TWO, bool ROWS32, bool PLAIN = false>
+// DEPENDENT: launched with programmatic stream serialisation, the set-up under the kernel before.
+template <int BN, bool TWO, bool ROWS32, bool PLAIN = false, bool DEPENDENT = false>
 __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const GemmParams& p,
                                           const int cta_first, const int cta_step) {
     using Cfg = GemmCfg<BN, TWO>;
@@ -429,6 +430,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     __syncthreads();
     if (TWO) cluster_sync_all();  // the partner's barriers exist before anything is signalled across the pair
     tc_fence_after();
+    if (DEPENDENT) { dependents_wait(); dependents_start(); }
     const uint32_t tmem_base = *tmem_slot;
 
     const int mn_tiles = p.m_tiles * p.n_tiles;  // TWO: m_tiles counts 256-row tiles of the pair
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 umma_gemm_two_kernel(const __grid_constant__ GemmTwoMaps maps, const __grid_constant__ GemmTwoParams tp) {
     const int unit = static_cast<int>(TWO ? blockIdx.x >> 1 : blockIdx.x), all = static_cast<int>(TWO ? gridDim.x >> 1 : gridDim.x);
     const int j = unit >= tp.units ? 1 : 0;
-    gemm_body<BN, TWO, false, PLAIN>(maps.a[j], maps.b[j], maps.c[j], tp.job[j], j ? unit - tp.units : unit, j ? all - tp.units : tp.units);
+    gemm_body<BN, TWO, false, PLAIN, true>(maps.a[j], maps.b[j], maps.c[j], tp.job[j], j ? unit - tp.units : unit, j ? all - tp.units : tp.units);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -2202,10 +2204,11 @@ static int launch_gemm_two(const GemmTwoMaps& maps, const GemmTwoParams& tp, int
     if (e != cudaSuccess) return set_cuda_error(e);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(TWO ? 2 * grid : grid); cfg.blockDim = dim3(GEMM_THREADS); cfg.dynamicSmemBytes = Cfg::SMEM_BYTES; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = TWO ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = TWO ? 2 : 1;
     return launched(cudaLaunchKernelEx(&cfg, umma_gemm_two_kernel<BN, TWO, PLAIN>, maps, tp));
 }
 int umma_gemm_two(const GemmCall& first, const GemmCall& second, const GemmTwoPlan& plan, cudaStream_t st) {
