@@ -15,10 +15,19 @@
 //
 // Sums of integers do not depend on their order, so tiles, splits and thread blocks change no bit of any result.
 //
-// Launches: vocab_stats_kernel (product + each piece's maximum and sum), vocab_entries_kernel (the logits of the wanted classes),
-// vocab_finish_kernel (row sums, loss, reciprocal, the errors of the wanted classes); for training, piece by piece of the
-// vocabulary, vocab_err_kernel (the product again, its errors as int8 in the workspace), vocab_patch_kernel and the two products
-// that lead back (umma_gemm), then the narrowing of the error.
+// Launches, each setting up under the one before:
+//   vocab_align_kernel     operands whose rows are no multiples of 16 bytes, copied to such a pitch
+//   vocab_kernel           the product; each piece's maximum and sum            (up to four tokens: vocab_thin_kernel)
+//   vocab_entries_kernel   a teacher's classes' logits
+//   vocab_finish_kernel    row sums, losses, reciprocals, the errors of the wanted classes
+// and for training, a piece of the vocabulary (up to 96 MB of errors) at a time,
+//   vocab_kernel           the product again, its errors as int8 into the workspace
+//   vocab_patch_kernel     a teacher's classes' errors over them
+//   umma_gemm_two          error and weight gradient                            (up to four tokens: vocab_back_thin_kernel)
+// and vocab_narrow_kernel, err_calc of the error.
+//
+// What bounds it: beyond a few hundred tokens vocab_kernel's epilogue up to about 2500 features (the integer pipes: E), the tensor
+// cores above; the two products the tensor cores; up to 128 tokens memory; a few small launches their number.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <climits>
@@ -99,7 +108,6 @@ struct VocabParams {
     int rows;                 // tokens
     int first, classes;       // of the piece of the vocabulary this launch covers (multiple of 256); classes of the whole vocabulary
     int32_t* piece_max; uint32_t* piece_sum;  // [pieces][rows]
-    const int* entries; int num_entries;      // a teacher's classes and their errors (one_entry), [num_entries][rows]; 0: none, or vocab_patch_kernel's
     const int4* row_stat;     // {M, R, n - 3, the wanted class where there is one: see one_entry}; R = 0: a row without an error
     int8_t* err; long long err_pitch;
     const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
@@ -391,11 +399,6 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 }
                 const int at = (stat.w & 0x3FFFF) - vp.first - col;
                 if ((stat.w & (1 << 23)) && at >= 0 && at < PIECE) out[at] = static_cast<int8_t>(stat.w >> 24);
-#pragma unroll 4
-                for (int k = 0; k < vp.num_entries; ++k) {
-                    const int w = __ldg(vp.entries + static_cast<long long>(k) * vp.rows + row), to = (w & 0x3FFFF) - vp.first - col;
-                    if ((w & (1 << 23)) && to >= 0 && to < PIECE) out[to] = static_cast<int8_t>(w >> 24);
-                }
             }
         }
     }
@@ -845,7 +848,8 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     }
 }
 
-// a teacher's entries in a piece of the vocabulary, over what vocab_kernel wrote there
+// A teacher's entries in a piece of the vocabulary, over what vocab_kernel wrote there.  (Looked through by vocab_kernel's epilogue, every
+// piece of 64 classes for itself, they cost 333 x 640 x 20011 with 50 entries 16 us more and won two with one.)
 __global__ void __launch_bounds__(256) vocab_patch_kernel(const int* entries, long long n, int rows, int first, int count, int8_t* err, long long pitch) {
     dependents_wait();
     dependents_start();
@@ -1356,11 +1360,6 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
 
     vp.row_stat = fp.row_stat;
     vp.err = err; vp.err_pitch = pl.piece;
-    // A teacher's entries are looked through by every piece of a row (about three operations each beside some twenty for each of its 64
-    // classes), or written by a launch of their own, 4 us a piece of the vocabulary: even at about 2^30 rows x classes x entries.
-    const bool patch = a->top != nullptr && static_cast<long long>(T) * pl.piece * K > (1ll << 30);
-    if (a->top != nullptr && !patch) { vp.entries = fp.entry_err; vp.num_entries = K; }
-    vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
     if (thin) {
         BackParams bp{};
         bp.logits = reinterpret_cast<const int32_t*>(ws + pl.logits_at);
@@ -1376,7 +1375,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         const int count = V - v0 < pl.piece ? V - v0 : pl.piece;
         vp.first = v0;
         if (int e = run_vocab(a->loss_round, x, w, T, F, pl.pitch, count, &vp, a->status, st)) return e;
-        if (patch) {
+        if (a->top != nullptr) {
             if (int e = launch_next(vocab_patch_kernel, dim3(static_cast<unsigned>((wanted + 255) / 256)), 256, 0, st, fp.entry_err, wanted, T, v0, count, vp.err, vp.err_pitch)) return e;
         }
         if (v0 > 0) plan = piece_calls(v0, count);
