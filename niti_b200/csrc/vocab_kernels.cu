@@ -1360,6 +1360,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
 
     vp.row_stat = fp.row_stat;
     vp.err = err; vp.err_pitch = pl.piece;
+    vp.seed = fp.seed; vp.rng_stream = a->loss_stream; vp.rng_offset = a->sample_offset;
     if (thin) {
         BackParams bp{};
         bp.logits = reinterpret_cast<const int32_t*>(ws + pl.logits_at);
