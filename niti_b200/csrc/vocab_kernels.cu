@@ -333,7 +333,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     } else {
         const int piece = (warp - 2) >> 2, q = warp & 3;  // its 64 columns and 32 rows of every tile
         const uint32_t abort_addr = smem_u32(const_cast<int*>(abort_flag));
-        const ExpScale sc = exp_scale(__ldg(vp.exp_x) + __ldg(vp.exp_w) - vp.temperature);
+        const ExpScale sc = exp_scale(*vp.exp_x + *vp.exp_w - vp.temperature);
         const uint32_t minus_unit = 0u - (1u << sc.sl);
         unsigned long long seed = 0;
         if (WHAT == ROUND_STOCHASTIC) seed = *vp.seed;
@@ -347,7 +347,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             const int col = n_t * BN + piece * PIECE;  // within this launch's classes
             const bool valid = row < vp.rows;
             int4 stat = make_int4(0, 0, 0, 0);
-            if (WHAT != VOCAB_STATS && valid) stat = __ldg(vp.row_stat + row);
+            if (WHAT != VOCAB_STATS && valid) stat = vp.row_stat[row];
             if (!mbar_wait_uniform(smem_u32(&tfull_bar[acc]), aph, abort_addr)) {
                 *abort_flag = 1;
                 if (lane == 0) report_abort(p.status, 4, 2);
@@ -418,8 +418,8 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 // Rows of `bytes` bytes, one behind the other from any address, to rows of a pitch of 16 bytes, the rest of each zeroed.  A thread to
 // 16 bytes: five aligned words and four funnel shifts; what lies across the tensor's ends is read byte by byte.
 // Two tensors with rows of the same length in one launch.
-__global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restrict__ src0, long long rows0, const int8_t* __restrict__ src1, long long rows1,
-                                                          uint4* __restrict__ dst0, uint4* __restrict__ dst1, int bytes, int pitch16) {
+__global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* src0, long long rows0, const int8_t* src1, long long rows1,
+                                                          uint4* dst0, uint4* dst1, int bytes, int pitch16) {
     const long long pieces0 = rows0 * pitch16, pieces = pieces0 + rows1 * pitch16;
     dependents_wait();
     dependents_start();
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restri
             const uint32_t shift = static_cast<uint32_t>(at - word0) * 8;
             uint32_t w[5];
 #pragma unroll
-            for (int k = 0; k < 5; ++k) w[k] = __ldg(p + k);
+            for (int k = 0; k < 5; ++k) w[k] = p[k];
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[k] = __funnelshift_r(w[k], w[k + 1], shift);
         } else {
@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(256) vocab_align_kernel(const int8_t* __restri
     }
 }
 // Every launch of a call may begin while the kernel before it ends (see dependents_wait, with which each of these kernels begins): a
-// training step of seven launches takes five to seven microseconds less.
+// training step of seven launches takes five to seven microseconds less. What an earlier launch wrote is read by plain loads: those through
+// the read-only path may be moved in front of the wait.
 template <class... P, class... A>
 int launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const A&... args) {
     cudaLaunchConfig_t cfg{};
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinPara
         const int c = i % p.chunks, t = i / p.chunks % T, copy = i / p.chunks / T;
         const int at = c * 16 - ((base + copy * p.step) & 15);  // the feature in the chunk's first byte
         if (ALIGNED && c * 16 + 16 <= p.F && (reinterpret_cast<uintptr_t>(p.x) | static_cast<uintptr_t>(p.x_pitch)) % 16 == 0) {
-            sx[i] = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.x_pitch) + c);
+            sx[i] = reinterpret_cast<const uint4*>(p.x + t * p.x_pitch)[c];
             continue;
         }
         uint32_t o[4] = {0, 0, 0, 0};
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinPara
             for (int c = lane; c < p.chunks; c += 32) {
                 uint4 v[THIN_ROWS];
 #pragma unroll
-                for (int r = 0; r < THIN_ROWS; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(at[r]) + c);
+                for (int r = 0; r < THIN_ROWS; ++r) v[r] = reinterpret_cast<const uint4*>(at[r])[c];
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
                     uint4 u = sx[t * p.chunks + c];
@@ -639,9 +640,9 @@ __global__ void __launch_bounds__(256) vocab_entries_kernel(const EntryParams p)
     }
 #pragma unroll 2
     for (int c = lane; c < p.F16; c += 32) {
-        const uint4 u = __ldg(a + c);
+        const uint4 u = a[c];
 #pragma unroll
-        for (int k = 0; k < ENTRIES_PER_WARP; ++k) sum[k] = dot16(u, __ldg(b[k] + c), sum[k]);
+        for (int k = 0; k < ENTRIES_PER_WARP; ++k) sum[k] = dot16(u, b[k][c], sum[k]);
     }
 #pragma unroll
     for (int k = 0; k < ENTRIES_PER_WARP; ++k) {
@@ -692,22 +693,22 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
         const int c = g + u * G;
         const bool in = there && c < p.pieces;
         const long long at = static_cast<long long>(c) * p.rows + row;
-        hm[u] = in ? __ldg(p.piece_max + at) : INT_MIN;
-        hs[u] = in ? __ldg(p.piece_sum + at) : 0u;
+        hm[u] = in ? p.piece_max[at] : INT_MIN;
+        hs[u] = in ? p.piece_sum[at] : 0u;
     }
-    const int e = __ldg(p.exp_x) + __ldg(p.exp_w) - p.temperature;
-    const long long mine = ONE && tid < RB && there ? __ldg(p.index + row) : -1;
+    const int e = *p.exp_x + *p.exp_w - p.temperature;
+    const long long mine = ONE && tid < RB && there ? p.index[row] : -1;
     if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) { *p.err_exp = p.temperature - 7; *p.clear[0] = 0; *p.clear[1] = 0; *p.clear[2] = 0; }
     for (long long i = static_cast<long long>(blockIdx.x) * FINISH_THREADS + tid; i < p.zero_count; i += static_cast<long long>(gridDim.x) * FINISH_THREADS)
         p.zero[i] = make_uint4(0, 0, 0, 0);
     if (ONE && warp < RB && row0 + warp < p.rows) {  // the wanted class's logit
-        const long long t = row0 + warp, j = __ldg(p.index + t);
+        const long long t = row0 + warp, j = p.index[t];
         if (j >= 0 && j < p.classes) {
             int sum = 0;
             if (p.x != nullptr) {
                 const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
 #pragma unroll 2
-                for (int c = lane; c < p.F16; c += 32) sum = dot16(__ldg(a + c), __ldg(b + c), sum);
+                for (int c = lane; c < p.F16; c += 32) sum = dot16(a[c], b[c], sum);
                 sum = __reduce_add_sync(0xFFFFFFFFu, sum);
             } else {
                 sum = p.logit[t];
@@ -722,7 +723,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     for (int u = 1; u < FINISH_HELD; ++u) m = max(m, hm[u]);
     if (there) {
 #pragma unroll 8
-        for (int c = g + FINISH_HELD * G; c < p.pieces; c += G) m = max(m, __ldg(p.piece_max + static_cast<long long>(c) * p.rows + row));
+        for (int c = g + FINISH_HELD * G; c < p.pieces; c += G) m = max(m, p.piece_max[static_cast<long long>(c) * p.rows + row]);
     }
     for (int o = RB; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if (lane < RB) s_max[warp][lane] = m;
@@ -746,8 +747,8 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
 #pragma unroll 4
         for (int c = g + FINISH_HELD * G; c < p.pieces; c += G) {
             const long long at = static_cast<long long>(c) * p.rows + row;
-            const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(__ldg(p.piece_max + at));
-            S += (static_cast<unsigned long long>(__ldg(p.piece_sum + at)) * exp_weight(d, sc)) >> 20;
+            const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(p.piece_max[at]);
+            S += (static_cast<unsigned long long>(p.piece_sum[at]) * exp_weight(d, sc)) >> 20;
         }
     }
     for (int o = RB; o < 32; o <<= 1) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
@@ -880,7 +881,7 @@ struct BackParams {
 __device__ int8_t error_of(int32_t a, const int4& stat, const ExpScale& sc, const BackParams& p, int t, int v) {
     if ((stat.w & (1 << 23)) && (stat.w & 0x3FFFF) == v) return static_cast<int8_t>(stat.w >> 24);
     for (int k = 0; k < p.num_entries; ++k) {
-        const int w = __ldg(p.entries + k * p.T + t);
+        const int w = p.entries[k * p.T + t];
         if ((w & (1 << 23)) && (w & 0x3FFFF) == v) return static_cast<int8_t>(w >> 24);
     }
     const uint32_t E = exp_weight(static_cast<unsigned>(stat.x) - static_cast<unsigned>(a), sc);
@@ -925,7 +926,7 @@ __global__ void __launch_bounds__(BACK_THREADS) vocab_back_thin_kernel(const Bac
         for (int i = tid; i < TQ * 4 * BACK_ROWS; i += BACK_THREADS) {
             const int t = i / BACK_ROWS, r = i % BACK_ROWS, v = v0 + r;
             int8_t e = 0;
-            if (t < p.T && v < p.V) e = error_of(__ldg(p.logits + static_cast<long long>(t) * p.V + v), __ldg(p.row_stat + t), sc, p, t, v);
+            if (t < p.T && v < p.V) e = error_of(p.logits[static_cast<long long>(t) * p.V + v], p.row_stat[t], sc, p, t, v);
             reinterpret_cast<int8_t*>(s_tokens)[r * TQ * 4 + t] = e;
             reinterpret_cast<int8_t*>(s_classes)[(r >> 2) * TQ * 16 + t * 4 + (r & 3)] = e;
         }
@@ -944,9 +945,9 @@ __global__ void __launch_bounds__(BACK_THREADS) vocab_back_thin_kernel(const Bac
 #pragma unroll
                     for (int j = 0; j < 4; j += VEC)
                         if (f[j] < p.F) {
-                            if (VEC == 4) row[k] = __ldg(reinterpret_cast<const uint32_t*>(at + f[j]));
-                            else if (VEC == 2) row[k] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(at + f[j]))) << (8 * j);
-                            else row[k] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(at + f[j]))) << (8 * j);
+                            if (VEC == 4) row[k] = *reinterpret_cast<const uint32_t*>(at + f[j]);
+                            else if (VEC == 2) row[k] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + f[j])) << (8 * j);
+                            else row[k] |= static_cast<uint32_t>(static_cast<uint8_t>(at[f[j]])) << (8 * j);
                         }
                 }
             }
