@@ -106,6 +106,7 @@ struct VocabParams {
     GemmParams g;
     const int32_t* exp_x; const int32_t* exp_w; int temperature;
     int rows;                 // tokens
+    int copies_log2;          // of the tokens in a row tile (see vocab_copies)
     int first, classes;       // of the piece of the vocabulary this launch covers (multiple of 256); classes of the whole vocabulary
     int32_t* piece_max; uint32_t* piece_sum;  // [pieces][rows]
     const int4* row_stat;     // {M, R, n - 3, the wanted class where there is one: see one_entry}; R = 0: a row without an error
@@ -131,7 +132,7 @@ struct VocabCfg {
 // the pace (2048 features: 12400 cycles a tile with the general roles, 8900 where the epilogue computed nothing).
 template <bool TWO, int BN>
 __device__ __forceinline__ void vocab_load(uint8_t* smem, uint64_t* full_bar, uint64_t* empty_bar, const CUtensorMap* tmA, const CUtensorMap* tmB,
-                                           const GemmParams& p, int first, int step, volatile int* abort_flag) {
+                                           const GemmParams& p, int copies_log2, int first, int step, volatile int* abort_flag) {
     using Cfg = VocabCfg<TWO, BN>;
     const int total = keep_reg(p.m_tiles * p.n_tiles), num_kb = keep_reg(p.num_kb);
     const uint32_t rank = TWO ? __shfl_sync(0xFFFFFFFFu, cluster_ctarank(), 0) : 0u;
@@ -161,7 +162,8 @@ __device__ __forceinline__ void vocab_load(uint8_t* smem, uint64_t* full_bar, ui
                     }
                 } else {
                     mbar_arrive_expect_tx(fb, block_tx);
-                    tma_load_2d(sa, tmA, fb, kb * ROW_BYTES, ya);
+#pragma unroll 1
+                    for (int c = 0; c < 1 << copies_log2; ++c) tma_load_2d(sa + c * (PANEL_BYTES >> copies_log2), tmA, fb, kb * ROW_BYTES, ya);
                     tma_load_2d(sa + PANEL_BYTES, tmB, fb, kb * ROW_BYTES, yb);
                 }
             }
@@ -324,7 +326,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     const int cta_step = TWO ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
     if (warp == 0) {
-        vocab_load<TWO, BN>(smem, full_bar, empty_bar, &tmA, &tmB, p, cta_first, cta_step, abort_flag);
+        vocab_load<TWO, BN>(smem, full_bar, empty_bar, &tmA, &tmB, p, vp.copies_log2, cta_first, cta_step, abort_flag);
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0)
@@ -343,9 +345,11 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             int m_pair, n_t;
             tile_coords(p, tile, &m_pair, &n_t);
             const int m_t = TWO ? 2 * m_pair + static_cast<int>(rank) : m_pair;
-            const int row = m_t * BLOCK_M + q * 32 + lane;
+            const int cl = TWO ? 0 : vp.copies_log2;
+            const int row = m_t * BLOCK_M + (q & ((4 >> cl) - 1)) * 32 + lane;
             const int col = n_t * BN + piece * PIECE;  // within this launch's classes
-            const bool valid = row < vp.rows;
+            const bool mine = ((piece + n_t) & ((1 << cl) - 1)) == q >> (2 - cl);  // this copy's rows see to these columns
+            const bool valid = mine && row < vp.rows;
             int4 stat = make_int4(0, 0, 0, 0);
             if (WHAT != VOCAB_STATS && valid) stat = vp.row_stat[row];
             if (!mbar_wait_uniform(smem_u32(&tfull_bar[acc]), aph, abort_addr)) {
@@ -356,7 +360,7 @@ vocab_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             tc_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN + piece * PIECE);
             uint32_t v[PIECE];
-            if (col < p.N) {
+            if (mine && col < p.N) {
                 tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
                 tmem_ld_32x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
                 tmem_ld_wait();
@@ -1147,27 +1151,34 @@ int launch_vocab(int what, const CUtensorMap& a, const CUtensorMap& b, const Voc
 // 128-byte reduction block of each; the first tile's blocks lie in front of every epilogue.  48 x 256 x 4096 (64 SMs instead of
 // 16): 11.8 -> 8.2 us; 333 x 640 x 20011 (939 tiles of 64 instead of three waves of pairs), the loss: 28.7 -> 22.6 us.
 struct VocabTile { int bn; bool pair; };
-VocabTile vocab_tile(int m128, int F, int count) {
+// A warp reads the tensor-memory lanes of its place in a group of four, which are the places on the four schedulers: 32 tokens' rows in
+// one quarter of a tile would leave all the work to one scheduler.  Up to 64 tokens lie in a tile twice, up to 32 four times, and
+// every copy's warps see to their share of the columns (the loss, 1024 features x 30000 classes: 32 tokens 18.6 -> 13.8 us, 64 18.6 ->
+// 14.6; 256 x 60000: 5 tokens 20.8 -> 13.4, 32 tokens 22.0 -> 17.4).
+int vocab_copies(int T) { return T <= 32 ? 2 : T <= 64 ? 1 : 0; }
+VocabTile vocab_tile(int T, int F, int count) {
+    const int m128 = (T + 127) / 128, wide_epilogue = 10400 >> vocab_copies(T);
     const long long kb = (F + 127) / 128, sms = sm_count();
     const bool pair = (g_two_cta & 1) && m128 >= 2;
     const auto larger = [](long long a, long long b) { return a > b ? a : b; };
     const long long wide = static_cast<long long>(pair ? (m128 + 1) / 2 : m128) * ((count + VBN - 1) / VBN), units = pair ? sms / 2 : sms, block = pair ? 600 : 700;
-    const long long wide_cost = kb * block + (wide + units - 1) / units * larger(10400, kb * block);
+    const long long wide_cost = kb * block + (wide + units - 1) / units * larger(wide_epilogue, kb * block);
     const long long narrow = static_cast<long long>(m128) * ((count + 63) / 64), whole = narrow / (2 * sms), rest = narrow - whole * 2 * sms;
-    const long long full = larger(5400, 2 * kb * 650), last = rest == 0 ? 0 : rest <= sms ? larger(4200, kb * 400) : full;
+    const long long full = larger(5400 >> (vocab_copies(T) != 0), 2 * kb * 650), last = rest == 0 ? 0 : rest <= sms ? larger(4200, kb * 400) : full;
     const long long narrow_cost = kb * 400 + whole * full + last;
     return narrow_cost < wide_cost ? VocabTile{64, false} : VocabTile{VBN, pair};
 }
 // x [T][pitch] times `count` rows of w [V][pitch] from p->first on
 int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitch, int count, VocabParams* p, int32_t* status, cudaStream_t st) {
     const int m128 = (T + 127) / 128;
-    const VocabTile tile = vocab_tile(m128, F, count);
+    const VocabTile tile = vocab_tile(T, F, count);
     const int bn = tile.bn;
     const bool pair = tile.pair;
     CUtensorMap ma, mb;
     uint64_t dims[2] = {static_cast<uint64_t>(F), static_cast<uint64_t>(T)}, str[1] = {static_cast<uint64_t>(pitch)};
     // a single row tile's box is no higher than its tokens (in eights): what the MMAs read of the other rows ends in rows nobody looks at
     const int a_rows = m128 == 1 ? (T + 7) / 8 * 8 : BLOCK_M;
+    p->copies_log2 = vocab_copies(T);
     uint32_t box[2] = {128, static_cast<uint32_t>(a_rows)};
     if (int e = encode_map(&ma, x, false, 2, dims, str, box)) return e;
     dims[1] = count; box[1] = pair ? VBN / 2 : bn;
@@ -1176,7 +1187,7 @@ int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitc
     g = GemmParams{};
     g.M = T; g.N = count; g.K = F; g.num_kb = (F + 127) / 128; g.splits = 1;
     g.m_tiles = pair ? (m128 + 1) / 2 : m128; g.n_tiles = (count + bn - 1) / bn;
-    g.a_bytes = a_rows * ROW_BYTES; g.status = status;
+    g.a_bytes = (a_rows << p->copies_log2) * ROW_BYTES; g.status = status;
     g.group_m = (static_cast<long long>(T) + count) * F > (48ll << 20) ? 8 : 0;  // as umma_gemm orders its tiles
     g.fd_mn = make_fastdiv(g.m_tiles * g.n_tiles); g.fd_n = make_fastdiv(g.n_tiles); g.fd_tw = make_fastdiv(1); g.fd_th = make_fastdiv(1);
     if (pair) return launch_vocab<true, VBN>(what, ma, mb, *p, st);

@@ -91,6 +91,18 @@ def test_train(T, F, V, mode):
     check_train(r, want)
 
 
+@pytest.mark.parametrize("F,V", [(80, 5003), (80, 45001), (2064, 1500)])
+@pytest.mark.parametrize("T", [5, 8, 31, 32, 33, 56, 63, 64, 65])
+def test_few_tokens_in_a_row_tile(T, F, V):
+    """Up to 64 tokens lie several times in a row tile: each row's every column is seen to once, in tiles of either width."""
+    rng, x, ex, w, ew, y = layer(T + F + V + 2, T, F, V)
+    y[T // 3] = -100
+    mode = [O.PSEUDO_STOCHASTIC, O.STOCHASTIC, O.ROUND][T % 3]
+    want = VO.vocab(x, ex, w, ew, y, loss_mode=mode, seed=77, sample_offset=1)
+    same_loss(ops.vocab_loss(cu(x), word(ex), cu(w), word(ew), cu(y)), want["loss"])
+    check_train(ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y), loss_mode=mode, seed=ops.seed_tensor(77, DEV), sample_offset=1), want)
+
+
 @pytest.mark.parametrize("kind", ["int8", "int32"])
 @pytest.mark.parametrize("T,F,V,K,temperature", [(1, 16, 1, 1, 0), (4, 32, 100, 3, 1), (40, 64, 300, 32, 0), (37, 96, 1000, 33, -1), (130, 128, 513, 64, 2),
                                                  (9, 20, 70, 128, 0), (300, 48, 90, 5, 3)])
