@@ -1149,7 +1149,8 @@ int launch_vocab(int what, const CUtensorMap& a, const CUtensorMap& b, const Voc
 // The tile of a launch: 256 columns of 128 rows (or of 256, to a pair of thread blocks), or 64 columns in up to three thread blocks to an SM,
 // for launches whose last wave of wide tiles would be far from full.  Cycles: an epilogue of 256 columns, one and two of 64 on an SM; a
 // 128-byte reduction block of each; the first tile's blocks lie in front of every epilogue.  48 x 256 x 4096 (64 SMs instead of
-// 16): 11.8 -> 8.2 us; 333 x 640 x 20011 (939 tiles of 64 instead of three waves of pairs), the loss: 28.7 -> 22.6 us.
+// 16): 11.8 -> 8.2 us.  A pair fetches half of w for each of its thread blocks, but computes a row tile for nothing where their number
+// is odd: training on 777 x 1000 x 10007 took 91.6 us in pairs (three waves) and takes 78.5 in single blocks (two).
 struct VocabTile { int bn; bool pair; };
 // A warp reads the tensor-memory lanes of its place in a group of four, which are the places on the four schedulers: 32 tokens' rows in
 // one quarter of a tile would leave all the work to one scheduler.  Up to 64 tokens lie in a tile twice, up to 32 four times, and
@@ -1159,14 +1160,16 @@ int vocab_copies(int T) { return T <= 32 ? 2 : T <= 64 ? 1 : 0; }
 VocabTile vocab_tile(int T, int F, int count) {
     const int m128 = (T + 127) / 128, wide_epilogue = 10400 >> vocab_copies(T);
     const long long kb = (F + 127) / 128, sms = sm_count();
-    const bool pair = (g_two_cta & 1) && m128 >= 2;
     const auto larger = [](long long a, long long b) { return a > b ? a : b; };
-    const long long wide = static_cast<long long>(pair ? (m128 + 1) / 2 : m128) * ((count + VBN - 1) / VBN), units = pair ? sms / 2 : sms, block = pair ? 600 : 700;
-    const long long wide_cost = kb * block + (wide + units - 1) / units * larger(wide_epilogue, kb * block);
+    const auto wide = [&](bool pair) {
+        const long long tiles = static_cast<long long>(pair ? (m128 + 1) / 2 : m128) * ((count + VBN - 1) / VBN), units = pair ? sms / 2 : sms, block = pair ? 600 : 700;
+        return kb * block + (tiles + units - 1) / units * larger(wide_epilogue, kb * block);
+    };
+    const long long single_cost = wide(false), pair_cost = (g_two_cta & 1) && m128 >= 2 ? wide(true) : single_cost + 1, wide_cost = pair_cost < single_cost ? pair_cost : single_cost;
     const long long narrow = static_cast<long long>(m128) * ((count + 63) / 64), whole = narrow / (2 * sms), rest = narrow - whole * 2 * sms;
     const long long full = larger(5400 >> (vocab_copies(T) != 0), 2 * kb * 650), last = rest == 0 ? 0 : rest <= sms ? larger(4200, kb * 400) : full;
     const long long narrow_cost = kb * 400 + whole * full + last;
-    return narrow_cost < wide_cost ? VocabTile{64, false} : VocabTile{VBN, pair};
+    return narrow_cost < wide_cost ? VocabTile{64, false} : VocabTile{VBN, pair_cost < single_cost};
 }
 // x [T][pitch] times `count` rows of w [V][pitch] from p->first on
 int run_vocab(int what, const int8_t* x, const int8_t* w, int T, int F, int pitch, int count, VocabParams* p, int32_t* status, cudaStream_t st) {
@@ -1337,7 +1340,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     FinishParams fp{};
     fp.exp_x = a->exp_x; fp.exp_w = a->exp_w; fp.exp_top = a->exp_top; fp.temperature = a->temperature_log2;
     fp.rows = T; fp.classes = V; fp.pieces = pl.pieces; fp.entries = K;
-    fp.rows_log2 = T >= 1024 ? 3 : T >= 256 ? 2 : 0;  // eight words of a piece fill a sector; few rows are better off in blocks of their own
+    fp.rows_log2 = T >= 2048 ? 3 : T >= 1024 ? 2 : T >= 256 ? 1 : 0;  // two to four blocks an SM, up to eight words of a piece: a sector
     fp.piece_max = vp.piece_max; fp.piece_sum = vp.piece_sum;
     fp.index = index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = logit; fp.loss = a->loss;
     if (a->top == nullptr && !thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
