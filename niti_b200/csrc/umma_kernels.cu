@@ -2180,18 +2180,23 @@ GemmTwoPlan umma_gemm_two_plan(const GemmCall& first, const GemmCall& second) {
     int t0, k0, t1, k1;
     gemm_extent(first, best.bn, best.pair, &t0, &k0);
     gemm_extent(second, best.bn, best.pair, &t1, &k1);
-    // waves of tiles times their reduction blocks and about six more (a tile's epilogue), the larger of the two
-    constexpr int PER_TILE = 6;
+    // Waves of tiles times their quarters of a reduction block (650 cycles), the larger of the two.  A tile's epilogue adds about six
+    // blocks.  Where what both share and the second's results go beyond the L2 (126 MB), a tile that is all epilogue takes eight and a
+    // half (128 KB of results leave an SM in 5400 cycles where all write), and a block of the first whose operand no other row tile reads
+    // waits for memory beside such writers.  Training on 16 tokens, 1024 x 50000: 117.4 -> 108.6 us, 2048 x 30000 123.1 -> 107.5; under the
+    // L2's size the two terms cost up to 2 % (512 x 20000: 38.6 -> 38.9).
+    const bool beyond_l2 = 5ll * first.N * first.K > (126ll << 20);
+    const int per_block = beyond_l2 && !best.pair && first.M <= BLOCK_M ? 10 : 4, least = beyond_l2 ? 34 : 0;
     long long best_cost = LLONG_MAX;
     const int cuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
     for (const int s : cuts) {
         if (s > 1 && 4 * s > k0) break;
-        const long long n0 = static_cast<long long>(t0) * s, c0 = (k0 + s - 1) / s + PER_TILE, c1 = k1 + PER_TILE;
+        const long long n0 = static_cast<long long>(t0) * s, c0 = static_cast<long long>((k0 + s - 1) / s) * per_block + 24, c1 = 4 * k1 + 24 > least ? 4 * k1 + 24 : least;
         const long long ideal = units * (n0 * c0) / (n0 * c0 + t1 * c1);
         for (long long u = ideal - 1; u <= ideal + 2; ++u) {
             long long u0 = u < 1 ? 1 : u > units - 1 ? units - 1 : u;
             if (n0 + t1 <= units) u0 = n0;
-            const long long u1 = units - u0, a = (n0 + u0 - 1) / u0 * c0, b = (t1 + u1 - 1) / u1 * c1, cost = (a > b ? a : b) + (s > 1 ? 2 : 0);
+            const long long u1 = units - u0, a = (n0 + u0 - 1) / u0 * c0, b = (t1 + u1 - 1) / u1 * c1, cost = (a > b ? a : b) + (s > 1 ? 8 : 0);
             if (cost < best_cost) { best_cost = cost; best.splits = s; best.units = static_cast<int>(u0 < n0 ? u0 : n0); best.grid = best.units + static_cast<int>(u1 < t1 ? u1 : t1); }
         }
     }
