@@ -183,7 +183,7 @@ def test_no_tokens():
 
 @pytest.mark.parametrize("T,F,V", [(70000, 32, 3000), (131071, 16, 1100)])
 def test_errors_that_take_several_pieces(T, F, V):
-    """More tokens than 64 MB of errors hold at once: adjointness and sums against the one-piece call on parts of the tokens."""
+    """More tokens than a piece of the errors holds at once: adjointness and sums against the one-piece call on parts of the tokens."""
     rng, x, ex, w, ew, y = layer(T, T, F, V)
     assert ops.vocab_pieces(T, V) > 1
     args = (word(ex), cu(w), word(ew))
@@ -201,6 +201,19 @@ def test_errors_that_take_several_pieces(T, F, V):
         a, b = part.double() * 2.0 ** e, e8[t:t + step].double() * 2.0 ** int(exp_err)
         assert float((a - b).abs().max()) <= 2.0 ** (e - 1) + 2.0 ** (int(exp_err) - 1)
     ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("cooperative", [True, False])
+@pytest.mark.parametrize("T,F,V", [(128, 1024, 800), (129, 1024, 800), (700, 250, 513)])
+def test_errors_about_the_size_that_one_cluster_narrows(T, F, V, cooperative):
+    rng, x, ex, w, ew, y = layer(T + F + V + 3, T, F, V)
+    want = VO.vocab(x, ex, w, ew, y, err_mode=O.STOCHASTIC, seed=8, sample_offset=5, err_stream=2)
+    old = ops.set_cooperative_launch(cooperative)
+    try:
+        r = ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y), err_mode=O.STOCHASTIC, seed=ops.seed_tensor(8, DEV), sample_offset=5, err_stream=2)
+    finally:
+        ops.set_cooperative_launch(old)
+    check_train(r, want)
 
 
 def test_results_do_not_depend_on_pairs_of_thread_blocks():
