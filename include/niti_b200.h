@@ -513,7 +513,7 @@ NITI_API int niti_fc_head_train_i8(const niti_fc_head_args* args, void* stream);
  *     have no entry, NaN where a class is not below V (or negative and not ignore_index); these rows have no error.
  * With g32 != null the gradients of the sum of the losses too (e8, exp_err, g32 and grad_maxabs are then required):
  *   err8 = p - q narrowed to int8 in units of 2^-7 by loss_round (a row of round_up(V, 4) random words of stream loss_stream per
- *     token where it is stochastic); what err_round, bits and err_stream say narrows the int32 error err8 W to e8 [T][F] as
+ *     token where it is stochastic); what err_round, bits (1 to 7) and err_stream say narrows the int32 error err8 W to e8 [T][F] as
  *     err_calc does (ti_torch.py:119-133), *exp_err = shift + *exp_w - 7 + temperature_log2;
  *   g32 [V][F] = err8^T x, *grad_maxabs = max |g32|, for niti_update_i8.
  *   sample_offset: global index of the first row, for the random words.

@@ -1327,6 +1327,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     if ((a->top == nullptr) != (a->exp_top == nullptr) || (a->top == nullptr && a->entries != 1)) return NITI_ERR_BAD_ARG;
     if (train && !(a->e8 && a->exp_err && a->grad_maxabs)) return NITI_ERR_BAD_ARG;
     if (train && (!aligned16(a->e8) || !aligned16(a->g32))) return NITI_ERR_BAD_ARG;
+    if (train && (a->bits < 1 || a->bits > 7)) return NITI_ERR_BAD_ARG;
     if (train && (a->loss_round < 0 || a->loss_round > 2 || a->err_round < 0 || a->err_round > 2 ||
                   (a->seed == nullptr && (a->loss_round == ROUND_STOCHASTIC || a->err_round == ROUND_STOCHASTIC))))
         return NITI_ERR_BAD_ARG;

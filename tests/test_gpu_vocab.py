@@ -283,6 +283,7 @@ def test_refusals():
         lambda: ops.vocab_distill_loss(x, ex, w, ew, idx.repeat(1, 33), top.repeat(1, 33), ex),
         lambda: ops.vocab_distill_loss(x, ex, w, ew, idx[:, :0], top[:, :0], ex),
         lambda: ops.vocab_train(x, ex, w, ew, y, loss_mode=1), lambda: ops.vocab_train(x, ex, w, ew, y, loss_mode=7), lambda: ops.vocab_train(x, ex, w, ew, y, err_mode=1),
+        lambda: ops.vocab_train(x, ex, w, ew, y, bits=0), lambda: ops.vocab_train(x, ex, w, ew, y, bits=8),
         lambda: ops.vocab_train(x, ex, w, ew, y, g32=torch.zeros((100, 31), dtype=torch.int32, device=DEV)),
         lambda: ops.vocab_train(x, ex, w, ew, y, g32=torch.zeros((100, 32), dtype=torch.int64, device=DEV)),
         lambda: ops.vocab_train(x, ex, w, ew, y, g32=torch.zeros(100 * 32 + 1, dtype=torch.int32, device=DEV)[1:].view(100, 32)),
