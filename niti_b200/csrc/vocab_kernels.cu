@@ -18,8 +18,7 @@
 // Launches, each setting up under the one before:
 //   vocab_align_kernel     operands whose rows are no multiples of 16 bytes, copied to such a pitch
 //   vocab_kernel           the product; each piece's maximum and sum            (up to four tokens: vocab_thin_kernel)
-//   vocab_entries_kernel   a teacher's classes' logits
-//   vocab_finish_kernel    row sums, losses, reciprocals, the errors of the wanted classes
+//   vocab_finish_kernel    the wanted classes' logits, row sums, losses, reciprocals, the wanted classes' errors
 // and for training, a piece of the vocabulary (up to 96 MB of errors) at a time,
 //   vocab_kernel           the product again, its errors as int8 into the workspace
 //   vocab_patch_kernel     a teacher's classes' errors over them
@@ -617,52 +616,15 @@ __global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinPara
     }
 }
 
-// ---------------------------------------------------------------------------------------------- wanted classes
-struct EntryParams {
-    const int8_t* x; const int8_t* w; int F16; int rows, classes, entries;
-    const long long* index;   // [rows][entries]: a class, or negative: none
-    int32_t* logit;           // [rows][entries]
-};
-// logit[t][k] = a[t][index[t][k]]: a warp to four entries of a row, 512 bytes of each operand at a time
-constexpr int ENTRIES_PER_WARP = 4;
-__global__ void __launch_bounds__(256) vocab_entries_kernel(const EntryParams p) {
-    const int groups = (p.entries + ENTRIES_PER_WARP - 1) / ENTRIES_PER_WARP;
-    dependents_wait();
-    dependents_start();
-    const long long i = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const long long row = i / groups;
-    if (row >= p.rows) return;
-    const int lane = threadIdx.x & 31, k0 = static_cast<int>(i - row * groups) * ENTRIES_PER_WARP;
-    const uint4* a = reinterpret_cast<const uint4*>(p.x) + row * p.F16;
-    const uint4* b[ENTRIES_PER_WARP];
-    int sum[ENTRIES_PER_WARP];
-#pragma unroll
-    for (int k = 0; k < ENTRIES_PER_WARP; ++k) {
-        const long long j = k0 + k < p.entries ? p.index[row * p.entries + k0 + k] : -1;
-        b[k] = reinterpret_cast<const uint4*>(p.w) + (j >= 0 && j < p.classes ? j : 0) * p.F16;  // any class where there is none: not looked at
-        sum[k] = 0;
-    }
-#pragma unroll 2
-    for (int c = lane; c < p.F16; c += 32) {
-        const uint4 u = a[c];
-#pragma unroll
-        for (int k = 0; k < ENTRIES_PER_WARP; ++k) sum[k] = dot16(u, b[k][c], sum[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < ENTRIES_PER_WARP; ++k) {
-        const int v = __reduce_add_sync(0xFFFFFFFFu, sum[k]);
-        if (lane == 0 && k0 + k < p.entries) p.logit[row * p.entries + k0 + k] = v;
-    }
-}
-
+// ---------------------------------------------------------------------------------------------- row sums and losses
 struct FinishParams {
     const int32_t* exp_x; const int32_t* exp_w; const int32_t* exp_top; int temperature;
     int rows, classes, pieces, entries, rows_log2;  // a block's rows: 2^rows_log2
     const int32_t* piece_max; const uint32_t* piece_sum;
     const long long* index; long long ignore;  // ignore: rows of this class are left out (a teacher's: every negative one is)
     const void* top; int top32;                // teacher's logits [rows][entries], int32 or int8; null: all on the one entry
-    int32_t* logit;                            // of the wanted classes; of a single one per row it is computed here
-    const int8_t* x; const int8_t* w; int F16; // null: they are all there
+    const int8_t* x; const int8_t* w; int F16; // for the wanted classes' logits; null: they lie in logit, [rows][entries]
+    const int32_t* logit;
     float* loss;
     int4* row_stat; int* entry_err;            // null: the loss alone; entry_err [entries][rows], see one_entry
     int32_t* err_exp; uint32_t* clear[3];      // training: written and zeroed for the launches behind
@@ -679,7 +641,7 @@ template <bool ONE>
 __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const FinishParams p) {
     constexpr int WARPS = FINISH_THREADS / 32, MAX_ROWS = 8;
     __shared__ unsigned long long s_sum[WARPS][MAX_ROWS];
-    __shared__ int32_t s_max[WARPS][MAX_ROWS], s_logit[MAX_ROWS];
+    __shared__ int32_t s_max[WARPS][MAX_ROWS], s_logit[MAX_ROWS][ONE ? 1 : MAX_ENTRIES];
     __shared__ unsigned s_share[ONE ? 1 : WARPS][ONE ? 1 : MAX_ENTRIES];
     __shared__ int s_class[ONE ? 1 : WARPS][ONE ? 1 : MAX_ENTRIES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -687,8 +649,44 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     const int r = tid & (RB - 1), g = tid >> p.rows_log2;
     const int row0 = static_cast<int>(blockIdx.x) << p.rows_log2, row = row0 + r;
     const bool there = row < p.rows;
+    // The wanted classes' logits, a warp to four of a row's: of tensors that were there before the launch in front of this one passed its
+    // own wait, so this one need not wait for it.  What a negative index or one behind the last class gets is not looked at.
+    constexpr int AT_ONCE = ONE ? 1 : 4;
+    if (p.x != nullptr) {
+        const int groups = (p.entries + AT_ONCE - 1) / AT_ONCE, tasks = groups << p.rows_log2;
+        for (int i = warp; i < tasks; i += WARPS) {
+            const int k0 = (i >> p.rows_log2) * AT_ONCE, ri = i & (RB - 1);
+            const long long t = row0 + ri;
+            if (t >= p.rows) continue;
+            const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b[AT_ONCE];
+            int sum[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const long long j = k0 + k < p.entries ? __ldcg(p.index + t * p.entries + k0 + k) : -1;
+                b[k] = reinterpret_cast<const uint4*>(p.w) + (j >= 0 && j < p.classes ? j : 0) * p.F16;
+                sum[k] = 0;
+            }
+#pragma unroll 2
+            for (int c = lane; c < p.F16; c += 32) {
+                uint4 v[AT_ONCE];
+                const uint4 u = __ldcg(a + c);
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) v[k] = __ldcg(b[k] + c);
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) sum[k] = dot16(u, v[k], sum[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int v = __reduce_add_sync(0xFFFFFFFFu, sum[k]);
+                if (lane == 0 && k0 + k < p.entries) s_logit[ri][k0 + k] = v;
+            }
+        }
+    }
     dependents_wait();
     dependents_start();
+    if (p.x == nullptr)
+        for (int i = tid; i < p.entries << p.rows_log2; i += FINISH_THREADS)
+            if (row0 + (i & (RB - 1)) < p.rows) s_logit[i & (RB - 1)][i >> p.rows_log2] = p.logit[static_cast<long long>(row0 + (i & (RB - 1))) * p.entries + (i >> p.rows_log2)];
 
     int32_t hm[FINISH_HELD];
     uint32_t hs[FINISH_HELD];
@@ -705,21 +703,6 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     if (p.err_exp != nullptr && blockIdx.x == 0 && tid == 0) { *p.err_exp = p.temperature - 7; *p.clear[0] = 0; *p.clear[1] = 0; *p.clear[2] = 0; }
     for (long long i = static_cast<long long>(blockIdx.x) * FINISH_THREADS + tid; i < p.zero_count; i += static_cast<long long>(gridDim.x) * FINISH_THREADS)
         p.zero[i] = make_uint4(0, 0, 0, 0);
-    if (ONE && warp < RB && row0 + warp < p.rows) {  // the wanted class's logit
-        const long long t = row0 + warp, j = p.index[t];
-        if (j >= 0 && j < p.classes) {
-            int sum = 0;
-            if (p.x != nullptr) {
-                const uint4 *a = reinterpret_cast<const uint4*>(p.x) + t * p.F16, *b = reinterpret_cast<const uint4*>(p.w) + j * p.F16;
-#pragma unroll 2
-                for (int c = lane; c < p.F16; c += 32) sum = dot16(a[c], b[c], sum);
-                sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-            } else {
-                sum = p.logit[t];
-            }
-            if (lane == 0) s_logit[warp] = sum;
-        }
-    }
 
     // the row's maximum over its pieces, then its sum relative to it
     int32_t m = hm[0];
@@ -766,7 +749,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) S += s_sum[w][tid];
         const bool used = mine >= 0 && mine < p.classes && mine != p.ignore, wrong = !used && mine != p.ignore;
-        const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(s_logit[tid]);
+        const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(s_logit[tid][0]);
         float loss = wrong ? __int_as_float(0x7FC00000) : 0.0f;
         if (used) loss = static_cast<float>(static_cast<double>(d) * unit + log(static_cast<double>(S) * pow2(-34)));
         p.loss[row] = loss;
@@ -824,7 +807,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     for (int k = lane; k < p.entries; k += 32) {
         const unsigned share = s_share[warp][k];
         if (share == 0) continue;
-        const double lnp = -(static_cast<double>(static_cast<long long>(Mi) - p.logit[first + k]) * unit + ln_s);
+        const double lnp = -(static_cast<double>(static_cast<long long>(Mi) - s_logit[i][k]) * unit + ln_s);
         const double lnq = -(static_cast<double>(static_cast<long long>(best) - teacher(k)) * teacher_unit + ln_q);
         loss += static_cast<double>(share) / static_cast<double>(total) * (lnq - lnp);
         s_share[warp][k] = static_cast<unsigned>((static_cast<unsigned long long>(share) << 30) / total);
@@ -844,7 +827,7 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
         if (learns) {
             unsigned q = 0;  // a class may be listed more than once
             for (int o = 0; o < p.entries; ++o) q += s_class[warp][o] == j ? s_share[warp][o] : 0u;
-            const uint32_t E = exp_weight(static_cast<unsigned>(Mi) - static_cast<unsigned>(p.logit[first + k]), sc);
+            const uint32_t E = exp_weight(static_cast<unsigned>(Mi) - static_cast<unsigned>(s_logit[i][k]), sc);
             const int32_t v = static_cast<int32_t>(mul_hi(E, R) >> sh) - static_cast<int32_t>(q);
             const unsigned long long at = (p.rng_offset + t) * static_cast<unsigned long long>((p.classes + 3) / 4 * 4) + j;
             err = narrow(v, 23, p.round_mode, p.round_mode == ROUND_STOCHASTIC ? random_word(seed, p.rng_stream, at) : 0u);
@@ -1105,9 +1088,10 @@ __global__ void __launch_bounds__(THREADS) vocab_narrow_kernel(const NarrowParam
     };
 #pragma unroll
     for (int u = 0; u < NARROW_HELD; ++u) if (first + u * step < words) emit(first + u * step, held[u]);
-    if (CLUSTER) return;
+    if constexpr (!CLUSTER) {
 #pragma unroll 2
-    for (long long i = first + NARROW_HELD * step; i < words; i += step) emit(i, load(i));
+        for (long long i = first + NARROW_HELD * step; i < words; i += step) emit(i, load(i));
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -1286,9 +1270,9 @@ VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
     const size_t t = T, k = entries;
     p.max_at = take(4 * t * p.pieces);
     p.sum_at = take(4 * t * p.pieces);
-    p.logit_at = take(4 * t * k);
-    p.word_at = take(16);
     const bool thin = thin_serves(T, F);
+    if (thin) p.logit_at = take(4 * t * k);
+    p.word_at = take(16);
     if (p.pitch != F && !thin) { p.x_at = take(t * p.pitch); p.w_at = take(static_cast<size_t>(V) * p.pitch); }
     if (train) {
         p.stat_at = take(16 * t);
@@ -1368,11 +1352,6 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     } else if (int e = run_vocab(VOCAB_STATS, x, w, T, F, pl.pitch, V, &vp, a->status, st)) {
         return e;
     }
-    if (a->top != nullptr && !thin) {
-        const EntryParams ep{x, w, pl.pitch / 16, T, V, K, index, logit};
-        const long long warps = static_cast<long long>(T) * ((K + ENTRIES_PER_WARP - 1) / ENTRIES_PER_WARP);
-        if (int e = launch_next(vocab_entries_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, st, ep)) return e;
-    }
 
     FinishParams fp{};
     fp.exp_x = a->exp_x; fp.exp_w = a->exp_w; fp.exp_top = a->exp_top; fp.temperature = a->temperature_log2;
@@ -1380,7 +1359,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     fp.rows_log2 = T >= 2048 ? 3 : T >= 1024 ? 2 : T >= 256 ? 1 : 0;  // two to four blocks an SM, up to eight words of a piece: a sector
     fp.piece_max = vp.piece_max; fp.piece_sum = vp.piece_sum;
     fp.index = index; fp.ignore = a->ignore_index; fp.top = a->top; fp.top32 = a->top_is_int32; fp.logit = logit; fp.loss = a->loss;
-    if (a->top == nullptr && !thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
+    if (!thin) { fp.x = x; fp.w = w; fp.F16 = pl.pitch / 16; }
     int32_t* words = reinterpret_cast<int32_t*>(ws + pl.word_at);  // {exponent of the logits' error, max |e32|, barrier}
     // e32 (+)= err w and g32 = err^T x of a piece of the vocabulary
     const int F4 = static_cast<int>(up(F, 4));
