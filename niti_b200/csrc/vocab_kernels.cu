@@ -1168,9 +1168,12 @@ int launch_vocab(int what, const CUtensorMap& a, const CUtensorMap& b, const Voc
 }
 // The tile of a launch: 256 columns of 128 rows (or of 256, to a pair of thread blocks), or 64 columns in up to three thread blocks to an SM,
 // for launches whose last wave of wide tiles would be far from full.  Cycles: an epilogue of 256 columns, one and two of 64 on an SM; a
-// 128-byte reduction block of each; the first tile's blocks lie in front of every epilogue.  48 x 256 x 4096 (64 SMs instead of
-// 16): 11.8 -> 8.2 us.  A pair fetches half of w for each of its thread blocks, but computes a row tile for nothing where their number
-// is odd: training on 777 x 1000 x 10007 took 91.6 us in pairs (three waves) and takes 78.5 in single blocks (two).
+// 128-byte reduction block of each; the first tile's blocks lie in front of every epilogue.  A box that the rows' end cuts short takes the
+// TMA unit 10 to 30 cycles a row.  48 x 256 x 4096 (64 SMs instead of 16): 11.8 -> 8.2 us.  In a graph, the loss in wide tiles and in
+// narrow ones: 128 x 128 x 8000 9.6 and 7.2 us, 128 x 128 x 17664 10.5 and 9.3, 200 x 128 x 60000 34.0 and 31.3; with part of a box 200 x
+// 80 x 60000 36.3 and 47.7, 200 x 400 x 17664 15.1 and 21.4; 32 x 128 x 17664 7.4 and 9.2.  A pair fetches half of w for each of its
+// thread blocks, but computes a row tile for nothing where their number is odd: training on 777 x 1000 x 10007 took 91.6 us in pairs
+// (three waves) and takes 78.5 in single blocks (two).
 struct VocabTile { int bn; bool pair; };
 // A warp reads the tensor-memory lanes of its place in a group of four, which are the places on the four schedulers: 32 tokens' rows in
 // one quarter of a tile would leave all the work to one scheduler.  Up to 64 tokens lie in a tile twice, up to 32 four times, and
@@ -1181,13 +1184,14 @@ VocabTile vocab_tile(int T, int F, int count) {
     const int m128 = (T + 127) / 128, wide_epilogue = 10400 >> vocab_copies(T);
     const long long kb = (F + 127) / 128, sms = sm_count();
     const auto larger = [](long long a, long long b) { return a > b ? a : b; };
+    const long long part = F % 128 != 0;  // the last box of a row is cut short
     const auto wide = [&](bool pair) {
-        const long long tiles = static_cast<long long>(pair ? (m128 + 1) / 2 : m128) * ((count + VBN - 1) / VBN), units = pair ? sms / 2 : sms, block = pair ? 600 : 700;
-        return kb * block + (tiles + units - 1) / units * larger(wide_epilogue, kb * block);
+        const long long tiles = static_cast<long long>(pair ? (m128 + 1) / 2 : m128) * ((count + VBN - 1) / VBN), units = pair ? sms / 2 : sms, load = kb * (pair ? 600 : 700);
+        return load + part * 1000 + wide_epilogue + (tiles - 1) / units * larger(wide_epilogue, load + part * (pair ? 3200 : 5000));
     };
     const long long single_cost = wide(false), pair_cost = (g_two_cta & 1) && m128 >= 2 ? wide(true) : single_cost + 1, wide_cost = pair_cost < single_cost ? pair_cost : single_cost;
     const long long narrow = static_cast<long long>(m128) * ((count + 63) / 64), whole = narrow / (2 * sms), rest = narrow - whole * 2 * sms;
-    const long long full = larger(5400 >> (vocab_copies(T) != 0), 2 * kb * 650), last = rest == 0 ? 0 : rest <= sms ? larger(4200, kb * 400) : full;
+    const long long full = larger(vocab_copies(T) != 0 ? 6000 : 5800, 2 * (kb * 650 + part * 5400)), last = rest == 0 ? 0 : rest <= sms ? larger(4200, kb * 400) + part * 2500 : full;
     const long long narrow_cost = kb * 400 + whole * full + last;
     return narrow_cost < wide_cost ? VocabTile{64, false} : VocabTile{VBN, pair_cost < single_cost};
 }
