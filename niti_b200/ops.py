@@ -415,9 +415,9 @@ def _vocab(train, x, w, index, *args):
     def work(r):
         (T, F), V = x.shape, w.shape[0]
         return (6 if train else 2) * T * V * F, T * F * (2 if train else 1) + V * F * (5 if train else 1) + 8 * index.numel() + 4 * T
-    # at most: operands in copies, statistics, wanted logits, row sums; the error's maximum and its narrowing; per piece of errors the
-    # product again, the wanted errors and the two products that lead back
-    launches = 5 if not train else 7 + 3 * vocab_pieces(max(1, x.size(0)), max(1, w.size(0)))
+    # at most: operands in copies, statistics, row sums; the error's maximum and its narrowing; per piece of errors the product again, the
+    # wanted errors and the two products that lead back
+    launches = 3 if not train else 5 + 3 * vocab_pieces(max(1, x.size(0)), max(1, w.size(0)))
     return _run("niti_vocab_loss_i8", launches, work, native.vocab_loss, *args)
 
 
