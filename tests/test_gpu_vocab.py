@@ -203,6 +203,44 @@ def test_errors_that_take_several_pieces(T, F, V):
     ops.check_status(DEV)
 
 
+@pytest.mark.parametrize("T", [2, 6, 40])
+def test_the_largest_vocabulary(T):
+    F, V = 48, 1 << 18
+    rng, x, ex, w, ew, y = layer(T, T, F, V)
+    y[0], y[1] = V - 1, 0
+    idx = np.stack([y, np.full(T, V - 1), rng.integers(0, V, T)], axis=1)
+    top = rng.integers(-9, 9, idx.shape).astype(np.int8)
+    check_train(ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y)), VO.vocab(x, ex, w, ew, y))
+    want = VO.vocab(x, ex, w, ew, idx, top=top, exp_top=-2, temperature_log2=1, loss_mode=O.STOCHASTIC, seed=3)
+    check_train(ops.vocab_distill_train(cu(x), word(ex), cu(w), word(ew), cu(idx), cu(top), word(-2), 1, loss_mode=O.STOCHASTIC, seed=ops.seed_tensor(3, DEV)), want)
+
+
+@pytest.mark.parametrize("T", [3, 5, 140])
+def test_the_longest_rows(T):
+    """Accumulators up to the ends of int32."""
+    F, V = 131071, 70
+    rng = np.random.default_rng(T)
+    x = rng.choice(np.array([-128, 127], np.int8), (T, 1)).repeat(F, 1)
+    w = rng.choice(np.array([-128, 127], np.int8), (V, 1)).repeat(F, 1)
+    x[0], w[1] = -128, -128
+    w[2, ::2] = 1
+    y = rng.integers(0, V, T)
+    for e in (-40, -31, -20):
+        check_train(ops.vocab_train(cu(x), word(e + 9), cu(w), word(-9), cu(y)), VO.vocab(x, e + 9, w, -9, y))
+
+
+def test_the_most_tokens_on_one_class():
+    """Sums over tokens up to the ends of int32."""
+    T, F, V = 131071, 16, 3
+    x, w = np.full((T, F), -128, np.int8), np.zeros((V, F), np.int8)
+    w[0] = 127
+    y = np.zeros(T, np.int64)
+    y[5] = 2
+    r = ops.vocab_train(cu(x), word(-4), cu(w), word(-4), cu(y))
+    check_train(r, VO.vocab(x, -4, w, -4, y))
+    assert int(r[4]) > 2 ** 30
+
+
 @pytest.mark.parametrize("cooperative", [True, False])
 @pytest.mark.parametrize("T,F,V", [(128, 1024, 800), (129, 1024, 800), (700, 250, 513)])
 def test_errors_about_the_size_that_one_cluster_narrows(T, F, V, cooperative):
@@ -243,6 +281,48 @@ def test_given_gradient_buffer_unaligned_views_and_other_streams():
         r = ops.vocab_train(cu(x), word(ex), cu(w), word(ew), cu(y))
     side.synchronize()
     check_train(r, want)
+
+
+@pytest.mark.parametrize("T,F,V", [(3, 64, 500), (40, 64, 3000), (300, 100, 2000)])
+def test_operands_written_right_before_a_call(T, F, V):
+    """Launches set up under the one before: what that one writes, the operands among it, is seen all the same, call after call."""
+    cases = []
+    for seed in (1, 2):
+        rng, x, ex, w, ew, y = layer(seed, T, F, V)
+        idx = rng.integers(0, V, (T, 5))
+        cases.append([cu(a) for a in (x, w, y, idx, rng.integers(-9, 9, (T, 5)).astype(np.int8))])
+    wants = [(ops.vocab_loss(x, word(ex), w, word(ew), y), ops.vocab_distill_loss(x, word(ex), w, word(ew), idx, top, word(-2)),
+              ops.vocab_train(x, word(ex), w, word(ew), y)) for x, w, y, idx, top in cases]
+    x, w, y, idx, top = (torch.empty_like(t) for t in cases[0])
+    exps = word(ex), word(ew), word(-2)
+    got = []
+    for i in range(40):
+        for to, frm in zip((x, w, y, idx, top), cases[i % 2]):
+            to.copy_(frm)
+        a = ops.vocab_loss(x, exps[0], w, exps[1], y)
+        b = ops.vocab_distill_loss(x, exps[0], w, exps[1], idx, top, exps[2])
+        got.append((a, b, ops.vocab_train(x, exps[0], w, exps[1], y)))
+    for i, (a, b, c) in enumerate(got):
+        want = wants[i % 2]
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1]) and all(torch.equal(u, v) for u, v in zip(c, want[2])), i
+
+
+def test_two_streams_at_once():
+    cases = []
+    for seed, (T, F, V) in enumerate([(500, 320, 6000), (30, 64, 9000)]):
+        rng, x, ex, w, ew, y = layer(seed, T, F, V)
+        cases.append((cu(x), word(ex), cu(w), word(ew), cu(y)))
+    wants = [ops.vocab_train(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], []
+    for _ in range(20):
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.vocab_train(*c))
+    torch.cuda.synchronize()
+    for i, r in enumerate(got):
+        assert all(torch.equal(u, v) for u, v in zip(r, wants[i % 2])), i
+    ops.check_status(DEV)
 
 
 def test_two_captured_steps_share_nothing():
