@@ -850,27 +850,27 @@ __global__ void __launch_bounds__(256) vocab_patch_kernel(const int* entries, lo
 // ---------------------------------------------------------------------------------------------- a few tokens' way back
 // Both products that lead back for the tokens of vocab_thin_kernel, from the logits it kept (no more bytes than a sixteenth of w's
 // features): w read once, the gradient written once, which is nearly all there is to do (an outer product of a few rows).  A thread
-// owns four features and walks the classes, four at a time: their errors with the features' tokens (dp4a over tokens) are the
-// gradient, which leaves at once; with w (dp4a over classes) they add up to the features' error, which is added to e32 at the
-// end.  2 x 1024 x 100000: 99 us, 5.2 TB/s; the tiles of umma_gemm_two, which are all epilogue here, 119 behind the 36 of
-// vocab_kernel (from five tokens on they are ahead: 8 x 1024 x 100000 with 16 tokens' room 161).
-constexpr int BACK_THREADS = 256, BACK_ROWS = 64, BACK_FEATURES = 4 * BACK_THREADS;
+// owns four features and sixteen classes of a batch, whose w it fetches at once (stores in between would hold the later ones back);
+// their errors with the features' tokens (dp4a over tokens) are the gradient, which leaves at once; with w (dp4a over classes) they add
+// up to the features' error, which is added to e32 at the end.  Rows shorter than 1024 features leave room for several groups of
+// sixteen classes in a block.  Training with one group and four classes at a time, and so: 2 x 256 x 89596 63.0 and 42.6 us, 1 x 64 x
+// 131072 48.1 and 27.7, 1 x 2048 x 30000 91.4 and 77.5.  Rows that are no multiple of four are fetched in up to four parts; four classes at
+// a time and four blocks an SM are ahead there (3 x 2046 x 20000: 120 us, sixteen at a time 136).  The tiles of umma_gemm_two, all epilogue
+// here, are ahead from five tokens on.
+constexpr int BACK_THREADS = 256, BACK_ROWS = 16, BACK_MIN_COLS = 32, BACK_MAX_GROUPS = BACK_THREADS / BACK_MIN_COLS;
 struct BackParams {
     const int32_t* logits;                    // [T][V]
     const int8_t* x; const int8_t* w;         // rows of F bytes
     int T, F, V, F4;
+    int cols_log2;                            // threads side by side along the features
     int32_t* e32; int32_t* g32; unsigned* g_max;
     const int32_t* exp_x; const int32_t* exp_w; int temperature;
     const int4* row_stat; const int* entries; int num_entries;
     int mode; const unsigned long long* seed; unsigned rng_stream; unsigned long long rng_offset;
 };
 // One class's error from its logit: what vocab_kernel computes, a value at a time.
-__device__ int8_t error_of(int32_t a, const int4& stat, const ExpScale& sc, const BackParams& p, int t, int v) {
+__device__ __forceinline__ int8_t error_of(int32_t a, const int4& stat, const ExpScale& sc, const BackParams& p, int t, int v) {
     if ((stat.w & (1 << 23)) && (stat.w & 0x3FFFF) == v) return static_cast<int8_t>(stat.w >> 24);
-    for (int k = 0; k < p.num_entries; ++k) {
-        const int w = p.entries[k * p.T + t];
-        if ((w & (1 << 23)) && (w & 0x3FFFF) == v) return static_cast<int8_t>(w >> 24);
-    }
     const uint32_t E = exp_weight(static_cast<unsigned>(stat.x) - static_cast<unsigned>(a), sc);
     const int32_t y = static_cast<int32_t>(mul_hi(E, static_cast<uint32_t>(stat.y)) >> stat.z);
     uint32_t rnd = 0;
@@ -878,57 +878,62 @@ __device__ int8_t error_of(int32_t a, const int4& stat, const ExpScale& sc, cons
     return narrow(y, 23, p.mode, rnd);
 }
 // VEC: features side by side that a thread loads and stores at once (4, or 2 or 1 where rows are no multiples of four)
+constexpr int back_per_sm(int vec) { return vec == 4 ? 2 : 4; }
 template <int NT, int VEC>
-__global__ void __launch_bounds__(BACK_THREADS) vocab_back_thin_kernel(const BackParams p) {
-    constexpr int TQ = (NT + 3) / 4;
-    __shared__ uint32_t s_tokens[BACK_ROWS][TQ];          // a class's errors, four tokens to a word
-    __shared__ uint32_t s_classes[BACK_ROWS / 4][TQ * 4]; // a token's errors, four classes to a word
+__global__ void __launch_bounds__(BACK_THREADS, back_per_sm(VEC)) vocab_back_thin_kernel(const BackParams p) {
+    constexpr int AT_ONCE = VEC == 4 ? BACK_ROWS : 4;  // classes whose w is fetched together
+    constexpr int MAX_ROWS = BACK_ROWS * BACK_MAX_GROUPS, TOKENS = 4, VALUES = MAX_ROWS * TOKENS / BACK_THREADS;
+    __shared__ uint32_t s_tokens[MAX_ROWS];             // a class's errors, a byte to each token
+    __shared__ uint32_t s_classes[MAX_ROWS / 4][TOKENS]; // a token's errors, four classes to a word
+    __shared__ int s_entries[MAX_ENTRIES * TOKENS], s_acc[NT * 4][BACK_THREADS];
     __shared__ unsigned s_max[BACK_THREADS / 32];
-    const int tid = threadIdx.x, f0 = static_cast<int>(blockIdx.y) * BACK_FEATURES;
+    const int tid = threadIdx.x, cols = 1 << p.cols_log2, ct = tid & (cols - 1), group = tid >> p.cols_log2;
+    const int rows_log2 = 4 + 8 - p.cols_log2, rows = 1 << rows_log2;  // classes of a batch: sixteen to each group
+    static_assert(BACK_ROWS == 16 && BACK_THREADS == 256, "rows_log2");
+    const int f0 = static_cast<int>(blockIdx.y) * 4 * cols;
     dependents_wait();
     dependents_start();
     const ExpScale sc = exp_scale(*p.exp_x + *p.exp_w - p.temperature);
+    for (int i = tid; i < p.num_entries * p.T; i += BACK_THREADS) s_entries[i] = p.entries[i];  // [entries][T]
     int f[4];
-    uint32_t xq[TQ][4];
+    uint32_t xq[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        f[j] = f0 + j / VEC * (VEC * BACK_THREADS) + VEC * tid + j % VEC;
+        f[j] = f0 + j / VEC * (VEC * cols) + VEC * ct + j % VEC;
+        xq[j] = 0;
 #pragma unroll
-        for (int q = 0; q < TQ; ++q) {
-            xq[q][j] = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (4 * q + k < p.T && f[j] < p.F) xq[q][j] |= static_cast<uint32_t>(static_cast<uint8_t>(p.x[static_cast<long long>(4 * q + k) * p.F + f[j]])) << (8 * k);
-        }
+        for (int k = 0; k < TOKENS; ++k)
+            if (k < p.T && f[j] < p.F) xq[j] |= static_cast<uint32_t>(static_cast<uint8_t>(p.x[static_cast<long long>(k) * p.F + f[j]])) << (8 * k);
     }
+    // a thread's errors of a batch: value u is class (tid + 256 u) % rows of token (tid + 256 u) / rows
+    int4 stat[VALUES];
+#pragma unroll
+    for (int u = 0; u < VALUES; ++u) {
+        const int t = (tid + u * BACK_THREADS) >> rows_log2;
+        stat[u] = t < p.T ? p.row_stat[t] : make_int4(0, 0, 0, 0);
+    }
+    const auto logit = [&](int u, int v0) {
+        const int i = tid + u * BACK_THREADS, t = i >> rows_log2, v = v0 + (i & (rows - 1));
+        return t < p.T && v < p.V ? p.logits[static_cast<long long>(t) * p.V + v] : 0;
+    };
     int acc[NT][4], hi = 0, lo = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[t][j] = 0;
-    const int batches = (p.V + BACK_ROWS - 1) / BACK_ROWS;
-    for (int batch = blockIdx.x; batch < batches; batch += gridDim.x) {
-        const int v0 = batch * BACK_ROWS;
-        __syncthreads();
-        for (int i = tid; i < TQ * 4 * BACK_ROWS; i += BACK_THREADS) {
-            const int t = i / BACK_ROWS, r = i % BACK_ROWS, v = v0 + r;
-            int8_t e = 0;
-            if (t < p.T && v < p.V) e = error_of(p.logits[static_cast<long long>(t) * p.V + v], p.row_stat[t], sc, p, t, v);
-            reinterpret_cast<int8_t*>(s_tokens)[r * TQ * 4 + t] = e;
-            reinterpret_cast<int8_t*>(s_classes)[(r >> 2) * TQ * 16 + t * 4 + (r & 3)] = e;
-        }
-        __syncthreads();
-        if (f[0] >= p.F) continue;
-#pragma unroll 2
-        for (int rq = 0; rq < BACK_ROWS / 4; ++rq) {
-            const int v = v0 + 4 * rq;
-            if (v >= p.V) break;
-            uint32_t row[4];
+    const int batches = (p.V + rows - 1) >> rows_log2;
+    int32_t a[VALUES];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+    for (int u = 0; u < VALUES; ++u) a[u] = logit(u, static_cast<int>(blockIdx.x) << rows_log2);
+    for (int batch = blockIdx.x; batch < batches; batch += gridDim.x) {
+        const int v0 = batch << rows_log2, mine = v0 + group * BACK_ROWS;
+        uint32_t row[AT_ONCE];
+        const auto fetch = [&](int first) {
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
                 row[k] = 0;
-                if (v + k < p.V) {
-                    const int8_t* at = p.w + static_cast<long long>(v + k) * p.F;
+                if (first + k < p.V) {
+                    const int8_t* at = p.w + static_cast<long long>(first + k) * p.F;
 #pragma unroll
                     for (int j = 0; j < 4; j += VEC)
                         if (f[j] < p.F) {
@@ -938,29 +943,54 @@ __global__ void __launch_bounds__(BACK_THREADS) vocab_back_thin_kernel(const Bac
                         }
                 }
             }
+        };
+        if (AT_ONCE == BACK_ROWS) fetch(mine);
+        __syncthreads();  // the batch before is done with the errors
+#pragma unroll
+        for (int u = 0; u < VALUES; ++u) {
+            const int i = tid + u * BACK_THREADS, t = i >> rows_log2, r = i & (rows - 1);
+            if (t >= TOKENS) break;
+            const int8_t e = t < p.T && v0 + r < p.V ? error_of(a[u], stat[u], sc, p, t, v0 + r) : int8_t(0);
+            reinterpret_cast<int8_t*>(s_tokens)[r * TOKENS + t] = e;
+            reinterpret_cast<int8_t*>(s_classes)[(r >> 2) * (4 * TOKENS) + t * 4 + (r & 3)] = e;
+            a[u] = logit(u, (batch + static_cast<int>(gridDim.x) < batches ? batch + static_cast<int>(gridDim.x) : batch) << rows_log2);
+        }
+        __syncthreads();
+        if (p.num_entries > 0) {  // a teacher's classes
+            for (int i = tid; i < p.num_entries * p.T; i += BACK_THREADS) {
+                const int w = s_entries[i], t = i % p.T, r = (w & 0x3FFFF) - v0;
+                if (!(w & (1 << 23)) || r < 0 || r >= rows) continue;
+                reinterpret_cast<int8_t*>(s_tokens)[r * TOKENS + t] = static_cast<int8_t>(w >> 24);
+                reinterpret_cast<int8_t*>(s_classes)[(r >> 2) * (4 * TOKENS) + t * 4 + (r & 3)] = static_cast<int8_t>(w >> 24);
+            }
+            __syncthreads();
+        }
+        if (f[0] >= p.F) continue;
+#pragma unroll (AT_ONCE / 4)
+        for (int rq = 0; rq < BACK_ROWS / 4; ++rq) {
+            if (AT_ONCE != BACK_ROWS) fetch(mine + 4 * rq);
             // four classes of a feature to a word
-            const uint32_t a = __byte_perm(row[0], row[1], 0x5140), b = __byte_perm(row[2], row[3], 0x5140);
-            const uint32_t c = __byte_perm(row[0], row[1], 0x7362), d = __byte_perm(row[2], row[3], 0x7362);
-            const uint32_t col[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x5410), __byte_perm(c, d, 0x7632)};
+            const uint32_t* four = row + (AT_ONCE == BACK_ROWS ? 4 * rq : 0);
+            const uint32_t b0 = __byte_perm(four[0], four[1], 0x5140), b1 = __byte_perm(four[2], four[3], 0x5140);
+            const uint32_t b2 = __byte_perm(four[0], four[1], 0x7362), b3 = __byte_perm(four[2], four[3], 0x7362);
+            const uint32_t col[4] = {__byte_perm(b0, b1, 0x5410), __byte_perm(b0, b1, 0x7632), __byte_perm(b2, b3, 0x5410), __byte_perm(b2, b3, 0x7632)};
+            const int rl = group * BACK_ROWS + 4 * rq;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const int e = static_cast<int>(s_classes[rq][t]);
+                const int e = static_cast<int>(s_classes[rl >> 2][t]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[t][j] = __dp4a(static_cast<int>(col[j]), e, acc[t][j]);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (v + k >= p.V) break;
-                int g[4] = {0, 0, 0, 0};
+                if (mine + 4 * rq + k >= p.V) break;
+                const int e = static_cast<int>(s_tokens[rl + k]);
+                int g[4];
 #pragma unroll
-                for (int q = 0; q < TQ; ++q) {
-                    const int e = static_cast<int>(s_tokens[4 * rq + k][q]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) g[j] = __dp4a(static_cast<int>(xq[q][j]), e, g[j]);
-                }
+                for (int j = 0; j < 4; ++j) g[j] = __dp4a(static_cast<int>(xq[j]), e, 0);
                 hi = __vimax3_s32(__vimax3_s32(hi, g[0], g[1]), g[2], g[3]);
                 lo = __vimin3_s32(__vimin3_s32(lo, g[0], g[1]), g[2], g[3]);
-                int32_t* to = p.g32 + static_cast<long long>(v + k) * p.F;
+                int32_t* to = p.g32 + static_cast<long long>(mine + 4 * rq + k) * p.F;
 #pragma unroll
                 for (int j = 0; j < 4; j += VEC)
                     if (f[j] < p.F) {
@@ -971,19 +1001,29 @@ __global__ void __launch_bounds__(BACK_THREADS) vocab_back_thin_kernel(const Bac
             }
         }
     }
+    // the groups' sums, then one addition a feature and token
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (t < p.T && f[j] < p.F && acc[t][j] != 0) atomicAdd(p.e32 + static_cast<long long>(t) * p.F4 + f[j], acc[t][j]);
+        for (int j = 0; j < 4; ++j) s_acc[t * 4 + j][tid] = acc[t][j];
     const unsigned m = __reduce_max_sync(0xFFFFFFFFu, max(static_cast<unsigned>(hi), static_cast<unsigned>(-lo)));
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
     __syncthreads();
-    if (tid == 0) {
-        unsigned x = 0;
+    if (group == 0) {
 #pragma unroll
-        for (int w = 0; w < BACK_THREADS / 32; ++w) x = max(x, s_max[w]);
-        if (x != 0) atomicMax(p.g_max, x);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                int sum = 0;
+                for (int i = ct; i < BACK_THREADS; i += cols) sum += s_acc[t * 4 + j][i];
+                if (t < p.T && f[j] < p.F && sum != 0) atomicAdd(p.e32 + static_cast<long long>(t) * p.F4 + f[j], sum);
+            }
+    }
+    if (tid == 0) {
+        unsigned largest = 0;
+#pragma unroll
+        for (int w = 0; w < BACK_THREADS / 32; ++w) largest = max(largest, s_max[w]);
+        if (largest != 0) atomicMax(p.g_max, largest);
     }
 }
 
@@ -1096,11 +1136,15 @@ __global__ void __launch_bounds__(THREADS) vocab_narrow_kernel(const NarrowParam
 
 // ---------------------------------------------------------------------------------------------- host side
 template <int NT>
-int launch_back_inst(const BackParams& p, cudaStream_t st) {
-    const int y = (p.F + BACK_FEATURES - 1) / BACK_FEATURES, batches = (p.V + BACK_ROWS - 1) / BACK_ROWS, most = (3 * sm_count() + y - 1) / y;
-    const dim3 grid(static_cast<unsigned>(batches < most ? batches : most), static_cast<unsigned>(y));
+int launch_back_inst(BackParams p, cudaStream_t st) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(p.w);
-    const auto kernel = p.F % 4 == 0 && at % 4 == 0 ? vocab_back_thin_kernel<NT, 4> : p.F % 2 == 0 && at % 2 == 0 ? vocab_back_thin_kernel<NT, 2> : vocab_back_thin_kernel<NT, 1>;
+    const int vec = p.F % 4 == 0 && at % 4 == 0 ? 4 : p.F % 2 == 0 && at % 2 == 0 ? 2 : 1;
+    int cols = BACK_MIN_COLS;
+    p.cols_log2 = 5;
+    while (cols < BACK_THREADS && 4 * cols < p.F) { cols *= 2; ++p.cols_log2; }
+    const int rows = BACK_ROWS * (BACK_THREADS / cols), y = (p.F + 4 * cols - 1) / (4 * cols), batches = (p.V + rows - 1) / rows, most = (back_per_sm(vec) * sm_count() + y - 1) / y;
+    const dim3 grid(static_cast<unsigned>(batches < most ? batches : most), static_cast<unsigned>(y));
+    const auto kernel = vec == 4 ? vocab_back_thin_kernel<NT, 4> : vec == 2 ? vocab_back_thin_kernel<NT, 2> : vocab_back_thin_kernel<NT, 1>;
     return launch_next(kernel, grid, BACK_THREADS, 0, st, p);
 }
 int launch_back(const BackParams& p, cudaStream_t st) {
