@@ -522,18 +522,52 @@ __global__ void __launch_bounds__(THIN_THREADS) vocab_thin_kernel(const ThinPara
     const int base = static_cast<int>(begin & 15);
     dependents_wait();
     dependents_start();
-    for (int i = tid; i < p.copies * T * p.chunks; i += THIN_THREADS) {
-        const int c = i % p.chunks, t = i / p.chunks % T, copy = i / p.chunks / T;
-        const int at = c * 16 - ((base + copy * p.step) & 15);  // the feature in the chunk's first byte
-        if (ALIGNED && c * 16 + 16 <= p.F && (reinterpret_cast<uintptr_t>(p.x) | static_cast<uintptr_t>(p.x_pitch)) % 16 == 0) {
-            sx[i] = reinterpret_cast<const uint4*>(p.x + t * p.x_pitch)[c];
-            continue;
-        }
-        uint32_t o[4] = {0, 0, 0, 0};
+    // The tokens' copies: as they are where rows are multiples of 16 bytes from such an address; otherwise five aligned words and four
+    // funnel shifts for a chunk, four chunks in flight, what lies outside the row zeroed (3 x 2046 x 20000: 43.7 us by bytes, 38.9 so).
+    if (ALIGNED) for (int i = tid; i < T * p.chunks; i += THIN_THREADS) sx[i] = reinterpret_cast<const uint4*>(p.x)[i];
+    const uintptr_t x_begin = reinterpret_cast<uintptr_t>(p.x), x_end = x_begin + static_cast<uintptr_t>(T - 1) * p.x_pitch + p.F;
+    const int chunks = p.copies * T * p.chunks;
+    constexpr int AT_ONCE = 4;
+    for (int i0 = tid; !ALIGNED && i0 < chunks; i0 += AT_ONCE * THIN_THREADS) {
+        uint32_t w[AT_ONCE][5], shift[AT_ONCE];
+        int at[AT_ONCE];  // the feature in the chunk's first byte
 #pragma unroll
-        for (int b = 0; b < 16; ++b)
-            if (at + b >= 0 && at + b < p.F) o[b >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p.x[t * p.x_pitch + at + b])) << (8 * (b & 3));
-        sx[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + u * THIN_THREADS;
+            if (i >= chunks) break;
+            const int c = i % p.chunks, t = i / p.chunks % T, copy = i / p.chunks / T;
+            at[u] = c * 16 - ((base + copy * p.step) & 15);
+            const uintptr_t from = x_begin + static_cast<uintptr_t>(t) * p.x_pitch + at[u], word0 = from & ~uintptr_t(3);
+            shift[u] = static_cast<uint32_t>(from - word0) * 8;
+            if (word0 >= x_begin && word0 + 20 <= x_end) {
+#pragma unroll
+                for (int k = 0; k < 5; ++k) w[u][k] = reinterpret_cast<const uint32_t*>(word0)[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 5; ++k) {
+                    w[u][k] = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const uintptr_t byte = word0 + 4 * k + b;
+                        if (byte >= x_begin && byte < x_end) w[u][k] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(byte)) << (8 * b);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + u * THIN_THREADS;
+            if (i >= chunks) break;
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int before = -at[u] - 4 * k, rest = p.F - at[u] - 4 * k;  // bytes in front of the row; bytes up to its end
+                o[k] = __funnelshift_r(w[u][k], w[u][k + 1], shift[u]);
+                if (before > 0) o[k] = before >= 4 ? 0u : o[k] & (0xFFFFFFFFu << (8 * before));
+                if (rest < 4) o[k] = rest <= 0 ? 0u : o[k] & ((1u << (8 * rest)) - 1u);
+            }
+            sx[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
     }
     const ExpScale sc = exp_scale(*p.exp_x + *p.exp_w - p.temperature);
     __syncthreads();
