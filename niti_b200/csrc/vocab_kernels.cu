@@ -1,5 +1,6 @@
 // A last layer with a vocabulary of classes and the losses over it: softmax cross entropy against one class a row and against a
-// teacher's top logits, with the error and the weight gradient, without the logits ever reaching memory.
+// teacher's top logits, with the error and the weight gradient, without the logits ever reaching memory (training on up to four
+// tokens keeps theirs).
 //
 // The reference ends in TiLinear.forward (ti_torch.py:241-253), TiLoss.forward (ti_loss.py:6-36) and TiLinear.backward (:255-266),
 // which write [rows][classes] logits and errors out and whose softmax has 11 bits: with 2048 equal classes every error is zero.
