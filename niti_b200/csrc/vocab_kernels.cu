@@ -1455,6 +1455,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         to_w = GemmCall{err, x, a->g32 + static_cast<long long>(v0) * F, a->grad_maxabs, count, F, T, 1, 0, 1, pl.piece, pl.pitch, F, 0, a->status};
         const GemmTwoPlan plan = umma_gemm_two_plan(to_x, to_w);
         if (plan.splits > 1) to_x.accumulate = 1;
+        if (plan.splits > 1 || pl.piece < V) to_x.maxabs = nullptr;  // a part's maximum is not the error's, which may be smaller
         return plan;
     };
     GemmTwoPlan plan{};
