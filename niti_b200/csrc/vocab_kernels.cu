@@ -1328,7 +1328,8 @@ int launch_thin(int T, const ThinParams& p, size_t smem, cudaStream_t st) {
     }
 }
 
-// The workspace of a call.
+// The workspace of a call, from the first 32-byte boundary on: vocab_kernel stores a row's errors 32 bytes at a time.
+constexpr size_t SCRATCH_ALIGN = 32, SCRATCH_SLACK = SCRATCH_ALIGN - 16;  // a caller's is 16-byte aligned
 struct VocabPlan {
     int pieces, pitch, piece;   // row pitch of the operands; classes whose errors are in the workspace at a time
     size_t max_at, sum_at, stat_at, logit_at, entry_at, err_at, e32_at, word_at, x_at, w_at, logits_at, bytes;
@@ -1364,7 +1365,7 @@ VocabPlan vocab_plan(int T, int F, int V, int entries, bool train) {
         else p.err_at = take(t * p.piece);
         p.e32_at = take(4 * t * up(F, 4));
     }
-    p.bytes = at;
+    p.bytes = at + SCRATCH_SLACK;
     return p;
 }
 
@@ -1403,7 +1404,7 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
     const VocabPlan pl = vocab_plan(T, F, V, K, train);
     if (!aligned16(a->scratch) || a->scratch_bytes < pl.bytes) return NITI_ERR_SCRATCH;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    char* ws = static_cast<char*>(a->scratch);
+    char* ws = reinterpret_cast<char*>(up(reinterpret_cast<uintptr_t>(a->scratch), SCRATCH_ALIGN));
 
     // operands whose rows are no multiples of 16 bytes go through copies that are
     const int8_t *x = a->x, *w = a->w;
