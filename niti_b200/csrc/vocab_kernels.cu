@@ -9,10 +9,15 @@
 //   a[t][v] = sum_f x[t][f] w[v][f],  e = exp_x + exp_w - temperature_log2
 //   E(d)    = 2^30 exp(-d 2^e) for whole d >= 0, in integers (exp_weight below; a quartic, |relative error| < 2.9e-6)
 //   pieces of 64 classes:  m_c = max a,  S_c = (sum E(m_c - a)) >> 6          (2^24 is 1)
-//   a row:  M = max m_c,  S = sum_c (S_c E(M - m_c)) >> 20                    (2^34 is 1)
-//   loss  = (M - a_y) 2^e + ln(S 2^-34)                                       (double, stored as float32)
+//   a row:  M = max m_c,  S = sum_c (S_c E(M - m_c)) >> 20                    (2^34 is 1; for p)
+//           L = sum_c (S_c q) >> (10 + I),  q >> I being E(M - m_c)           (2^44 is 1; for the loss)
+//   loss  = (M - a_y) 2^e + ln(L 2^-44)                                       (double, stored as float32)
 //   p     = hi32(E(M - a) R) >> (n - 3),  R = (2^63 - 1) / (S >> n), 2^31 <= S >> n < 2^32    (2^30 is 1; S >= 2^34, so n >= 3)
 //   err   = p - target share, narrowed by 23 bits to int8 (2^-7), NITI's roundings
+//
+// E ends at 2^-30, so S loses up to 2^-30 of each class of a piece far below the maximum: p is up to V 2^-30 (2.4e-4 for 2^18 classes) of
+// itself too large, a thirtieth of err's unit.  As a loss that would be all there is where one class stands alone (16 nats above 131072
+// others 0.7 % of it, from 21.5 on everything), so L shifts the product, not E.
 //
 // Sums of integers do not depend on their order, so tiles, splits and thread blocks change no bit of any result.
 //
@@ -76,17 +81,33 @@ __device__ __forceinline__ uint32_t shift_right(uint32_t a, uint32_t n) {  // 0 
     asm("shr.u32 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(n));
     return d;
 }
-// xs = min(d, D) << sl
-__device__ __forceinline__ uint32_t exp_weight_shifted(uint32_t xs, uint32_t K) {
-    const uint32_t h = mul_hi(xs, K);
+// E before its shift; h: u without its half
+__device__ __forceinline__ uint32_t exp_mantissa(uint32_t h) {
     const int32_t phi = static_cast<int32_t>(h << 7);  // the fraction of h + 2^24, less a half, with 2^32 as 1
     int32_t q = mul_hi(phi, 10289510) - 60029066;
     q = mul_hi(phi, q) + 257956795;
     q = mul_hi(phi, q) - 744236436;
-    q = mul_hi(phi, q) + (1 << 30);
-    return shift_right(static_cast<uint32_t>(q), (h + (1u << 24)) >> 25);
+    return static_cast<uint32_t>(mul_hi(phi, q) + (1 << 30));
+}
+// xs = min(d, D) << sl
+__device__ __forceinline__ uint32_t exp_weight_shifted(uint32_t xs, uint32_t K) {
+    const uint32_t h = mul_hi(xs, K);
+    return shift_right(exp_mantissa(h), (h + (1u << 24)) >> 25);
 }
 __device__ __forceinline__ uint32_t exp_weight(uint32_t d, const ExpScale& s) { return exp_weight_shifted(min(d, s.D) << s.sl, s.K); }
+
+// The largest d that a row's sums tell from no term at all: 64 nats and more, where d 2^(26+e) has 32 bits.  Of units above 32 nats (which
+// exp_scale takes for 32) it is 0.
+__device__ __forceinline__ unsigned far_limit(int e, const ExpScale& s) { return e > 5 ? 0u : 0xFFFFFFFFu >> s.sl; }
+// A piece's part of its row's sums; S is for training alone.  No branch, which would hold back the loads behind it: beside one sum of
+// cut E's, the two cost 8192 x 1024 x 32768 with an early return 5 us of 337, this way nothing that shows.
+template <bool TRAIN>
+__device__ __forceinline__ void add_piece(uint32_t sum, uint32_t d, const ExpScale& s, unsigned far, unsigned long long* S, unsigned long long* L) {
+    if (d > far) sum = 0;
+    const uint32_t h = mul_hi(min(d, far) << s.sl, s.K), q = exp_mantissa(h), I = (h + (1u << 24)) >> 25;
+    if (TRAIN) *S += (static_cast<unsigned long long>(sum) * shift_right(q, I)) >> 20;
+    *L += (static_cast<unsigned long long>(sum) * q) >> min(10u + I, 63u);  // 30 and 31 bits: none is left behind 63
+}
 
 // A row's view of E: E(M - a) for its accumulators a <= M.  max(a, floor) cuts d at D; the difference is taken in the
 // multiply-add that shifts it (modulo 2^32, which the result stays below).
@@ -661,7 +682,7 @@ struct FinishParams {
     const int8_t* x; const int8_t* w; int F16; // for the wanted classes' logits; null: they lie in logit, [rows][entries]
     const int32_t* logit;
     float* loss;
-    int4* row_stat; int* entry_err;            // null: the loss alone; entry_err [entries][rows], see one_entry
+    int4* row_stat; int* entry_err;            // training; entry_err [entries][rows], see one_entry
     int32_t* err_exp; uint32_t* clear[3];      // training: written and zeroed for the launches behind
     uint4* zero; long long zero_count;         // training: zeroed as well
     int round_mode;
@@ -672,10 +693,10 @@ __device__ __forceinline__ double pow2(int e) { return __hiloint2double((1023 + 
 // piece of one of them, the first eight at once and into registers, so that a short vocabulary costs one trip to memory.
 // ONE: a class to each row, finished by a thread; otherwise a warp to each row, its lanes to the entries.
 constexpr int FINISH_HELD = 8;
-template <bool ONE>
+template <bool ONE, bool TRAIN>
 __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const FinishParams p) {
     constexpr int WARPS = FINISH_THREADS / 32, MAX_ROWS = 8;
-    __shared__ unsigned long long s_sum[WARPS][MAX_ROWS];
+    __shared__ unsigned long long s_sum[WARPS][MAX_ROWS], s_loss_sum[WARPS][MAX_ROWS];
     __shared__ int32_t s_max[WARPS][MAX_ROWS], s_logit[MAX_ROWS][ONE ? 1 : MAX_ENTRIES];
     __shared__ unsigned s_share[ONE ? 1 : WARPS][ONE ? 1 : MAX_ENTRIES];
     __shared__ int s_class[ONE ? 1 : WARPS][ONE ? 1 : MAX_ENTRIES];
@@ -755,7 +776,8 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     for (int w = 1; w < WARPS; ++w) m = max(m, s_max[w][r]);
     const int32_t M = m;
     const ExpScale sc = exp_scale(e);
-    unsigned long long S = 0;
+    const unsigned far = far_limit(e, sc);
+    unsigned long long S = 0, L = 0;
 #pragma unroll 1
     for (int u = 0; u < FINISH_HELD; ++u) {
         // (a loop around one copy of E: this code runs once, and what a thread block has to fetch of it takes longer than it runs)
@@ -763,32 +785,34 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
 #pragma unroll
         for (int k = 1; k < FINISH_HELD; ++k) if (k == u) { mu = hm[k]; su = hs[k]; }
         if (g + u * G >= p.pieces) break;
-        S += (static_cast<unsigned long long>(su) * exp_weight(static_cast<unsigned>(M) - static_cast<unsigned>(mu), sc)) >> 20;
+        add_piece<TRAIN>(su, static_cast<unsigned>(M) - static_cast<unsigned>(mu), sc, far, &S, &L);
     }
     if (there) {
 #pragma unroll 4
         for (int c = g + FINISH_HELD * G; c < p.pieces; c += G) {
             const long long at = static_cast<long long>(c) * p.rows + row;
-            const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(p.piece_max[at]);
-            S += (static_cast<unsigned long long>(p.piece_sum[at]) * exp_weight(d, sc)) >> 20;
+            add_piece<TRAIN>(p.piece_sum[at], static_cast<unsigned>(M) - static_cast<unsigned>(p.piece_max[at]), sc, far, &S, &L);
         }
     }
-    for (int o = RB; o < 32; o <<= 1) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
-    if (lane < RB) s_sum[warp][lane] = S;
+    for (int o = RB; o < 32; o <<= 1) {
+        if (TRAIN) S += __shfl_xor_sync(0xFFFFFFFFu, S, o);
+        L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
+    }
+    if (lane < RB) { s_sum[warp][lane] = S; s_loss_sum[warp][lane] = L; }
     __syncthreads();
 
     const double unit = pow2(e);
     if (ONE) {
         if (tid >= RB || !there) return;
-        S = 0;
+        S = L = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) S += s_sum[w][tid];
+        for (int w = 0; w < WARPS; ++w) { S += s_sum[w][tid]; L += s_loss_sum[w][tid]; }
         const bool used = mine >= 0 && mine < p.classes && mine != p.ignore, wrong = !used && mine != p.ignore;
         const unsigned d = static_cast<unsigned>(M) - static_cast<unsigned>(s_logit[tid][0]);
         float loss = wrong ? __int_as_float(0x7FC00000) : 0.0f;
-        if (used) loss = static_cast<float>(static_cast<double>(d) * unit + log(static_cast<double>(S) * pow2(-34)));
+        if (used) loss = static_cast<float>(static_cast<double>(d) * unit + log(static_cast<double>(L) * pow2(-44)));
         p.loss[row] = loss;
-        if (p.row_stat == nullptr) return;
+        if (!TRAIN) return;
         const int n = 32 - __clzll(static_cast<long long>(S));
         const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (S >> n)), sh = static_cast<uint32_t>(n - 3);
         int one = 0;
@@ -804,12 +828,10 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     // a teacher's entries: a warp to each row
     const int i = warp, t = row0 + warp;
     if (i >= RB || t >= p.rows) return;
-    unsigned long long Si = 0;
+    unsigned long long Si = 0, Li = 0;
     int32_t Mi = INT_MIN;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) { Si += s_sum[w][i]; Mi = max(Mi, s_max[w][i]); }
-    const int n = 32 - __clzll(static_cast<long long>(Si));
-    const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (Si >> n)), sh = static_cast<uint32_t>(n - 3);
+    for (int w = 0; w < WARPS; ++w) { Si += s_sum[w][i]; Li += s_loss_sum[w][i]; Mi = max(Mi, s_max[w][i]); }
     const long long first = static_cast<long long>(t) * p.entries;
     const int et = *p.exp_top - p.temperature;
     const ExpScale st = exp_scale(et);
@@ -837,12 +859,12 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
         total += share;
     }
     total = warp_sum(total);
-    const double ln_s = log(static_cast<double>(Si) * pow2(-34)), ln_q = log(static_cast<double>(total) * pow2(-30)), teacher_unit = pow2(et);
+    const double ln_l = log(static_cast<double>(Li) * pow2(-44)), ln_q = log(static_cast<double>(total) * pow2(-30)), teacher_unit = pow2(et);
     double loss = 0.0;
     for (int k = lane; k < p.entries; k += 32) {
         const unsigned share = s_share[warp][k];
         if (share == 0) continue;
-        const double lnp = -(static_cast<double>(static_cast<long long>(Mi) - s_logit[i][k]) * unit + ln_s);
+        const double lnp = -(static_cast<double>(static_cast<long long>(Mi) - s_logit[i][k]) * unit + ln_l);
         const double lnq = -(static_cast<double>(static_cast<long long>(best) - teacher(k)) * teacher_unit + ln_q);
         loss += static_cast<double>(share) / static_cast<double>(total) * (lnq - lnp);
         s_share[warp][k] = static_cast<unsigned>((static_cast<unsigned long long>(share) << 30) / total);
@@ -850,7 +872,9 @@ __global__ void __launch_bounds__(FINISH_THREADS) vocab_finish_kernel(const Fini
     loss = warp_sum(loss) * pow2(2 * p.temperature);
     const bool learns = any && !wrong;
     if (lane == 0) p.loss[t] = wrong ? __int_as_float(0x7FC00000) : any ? static_cast<float>(loss) : 0.0f;
-    if (p.row_stat == nullptr) return;
+    if (!TRAIN) return;
+    const int n = 32 - __clzll(static_cast<long long>(Si));
+    const uint32_t R = static_cast<uint32_t>(((1ull << 63) - 1) / (Si >> n)), sh = static_cast<uint32_t>(n - 3);
     if (lane == 0) p.row_stat[t] = make_int4(Mi, learns ? static_cast<int32_t>(R) : 0, static_cast<int32_t>(sh), 0);
     __syncwarp();
     const unsigned long long seed = p.round_mode == ROUND_STOCHASTIC ? *p.seed : 0;
@@ -1471,7 +1495,9 @@ extern "C" int niti_vocab_loss_i8(const niti_vocab_args* a, void* stream) {
         fp.seed = reinterpret_cast<const unsigned long long*>(a->seed); fp.rng_stream = a->loss_stream; fp.rng_offset = a->sample_offset;
     }
     const int rb = 1 << fp.rows_log2;
-    if (int e = launch_next(a->top == nullptr ? vocab_finish_kernel<true> : vocab_finish_kernel<false>, dim3(static_cast<unsigned>((T + rb - 1) / rb)), FINISH_THREADS, 0, st, fp)) return e;
+    const auto finish = a->top == nullptr ? (train ? vocab_finish_kernel<true, true> : vocab_finish_kernel<true, false>)
+                                          : (train ? vocab_finish_kernel<false, true> : vocab_finish_kernel<false, false>);
+    if (int e = launch_next(finish, dim3(static_cast<unsigned>((T + rb - 1) / rb)), FINISH_THREADS, 0, st, fp)) return e;
     if (!train) return NITI_OK;
 
     vp.row_stat = fp.row_stat;

@@ -15,6 +15,17 @@ LOG2E_31 = 0xB8AA3B29  # round(log2(e) * 2**31)
 COEFF = (1 << 30, -744236436, 257956795, -60029066, 10289510)  # 2**-phi * 2**30, phi in [-1/2, 1/2)
 
 
+def _mantissas(d, e):
+    """(q, I): E(d) is q >> I.  d 2**e below 64."""
+    up, down = max(0, 26 + e), max(0, -26 - e)
+    u = ((d << up).astype(np.uint64) * np.uint64(LOG2E_31 >> down) >> np.uint64(32)).astype(np.int64) + (1 << 24)
+    phi = ((u & ((1 << 25) - 1)) - (1 << 24)) << 7
+    q = np.full_like(phi, COEFF[4])
+    for c in COEFF[3::-1]:
+        q = (phi * q >> 32) + c
+    return q, u >> 25
+
+
 def exp_weights(d, e):
     """E(d) = 2**30 exp(-d 2**e) for an int64 array d >= 0 and a Python int e."""
     d = np.asarray(d, dtype=np.int64)
@@ -25,13 +36,8 @@ def exp_weights(d, e):
         cut = (1 << 32) - 1
     else:
         cut = 43 << (-e - 1)
-    up, down = max(0, 26 + e), max(0, -26 - e)
-    u = ((np.minimum(d, cut) << up) * (LOG2E_31 >> down) >> 32) + (1 << 24)
-    phi = ((u & ((1 << 25) - 1)) - (1 << 24)) << 7
-    q = np.full_like(phi, COEFF[4])
-    for c in COEFF[3::-1]:
-        q = (phi * q >> 32) + c
-    return np.where(u >> 25 < 63, q >> np.minimum(u >> 25, 63), 0)
+    q, I = _mantissas(np.minimum(d, cut), e)
+    return np.where(I < 63, q >> np.minimum(I, 63), 0)
 
 
 def row_statistics(acc, e):
@@ -45,6 +51,22 @@ def row_statistics(acc, e):
         part = exp_weights(m[:, None] - a, e).sum(1) >> 6
         S += part * exp_weights(M - m, e) >> 20
     return M, S
+
+
+def row_loss_sums(acc, e):
+    """Each row's sum of exponentials for its loss, with 2**44 as 1: the pieces' sums are scaled by exponentials that are not cut to
+    units of 2**-30 first."""
+    acc = acc.astype(np.int64)
+    M, e = acc.max(1), int(e)
+    L = np.zeros(len(acc), dtype=np.int64)
+    for c in range(0, acc.shape[1], PIECE):
+        a = acc[:, c:c + PIECE]
+        m = a.max(1)
+        part, d = exp_weights(m[:, None] - a, e).sum(1) >> 6, M - m
+        there = d <= (0 if e > 5 else (1 << 32) - 1 >> max(0, 26 + e))  # 64 nats; units of more than 32 nats tell 0 from the rest
+        q, I = _mantissas(np.where(there, d, 0), min(e, 5))
+        L += np.where(there, part * q >> np.minimum(10 + I, 63), 0)
+    return L
 
 
 def probabilities(acc, M, S, e):
@@ -64,6 +86,7 @@ def vocab(x, exp_x, w, exp_w, index, ignore_index=-100, top=None, exp_top=0, tem
     acc = x.astype(np.int64) @ w.astype(np.int64).T
     e = exp_x + exp_w - temperature_log2
     M, S = row_statistics(acc, e)
+    L = row_loss_sums(acc, e)
     index = index.reshape(T, -1)
     loss = np.zeros(T)
     learns = np.zeros(T, dtype=bool)
@@ -84,11 +107,11 @@ def vocab(x, exp_x, w, exp_w, index, ignore_index=-100, top=None, exp_top=0, tem
             share = [int(exp_weights(best - int(b[k]), exp_top - temperature_log2)) for k in used]
             lnq = [-(best - int(b[k])) * 2.0 ** (exp_top - temperature_log2) - math.log(sum(share) / 2.0 ** 30) for k in used]
         total = sum(share)
-        lns = math.log(int(S[t]) / 2.0 ** 34)
+        lnl = math.log(int(L[t]) / 2.0 ** 44)
         for k, s, l in zip(used, share, lnq):
             j = int(index[t, k])
             if s:
-                loss[t] += s / total * ((int(M[t]) - int(acc[t, j])) * 2.0 ** e + lns + l)
+                loss[t] += s / total * ((int(M[t]) - int(acc[t, j])) * 2.0 ** e + lnl + l)
             want[t, j] += (s << 30) // total
         loss[t] *= 4.0 ** temperature_log2
     r = {"loss": loss}
