@@ -420,7 +420,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         fence_barrier_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
-        tma_prefetch_desc(&tmC);
+        if (!PLAIN || p.plain_out == nullptr) tma_prefetch_desc(&tmC);  // (there is no map of a result that leaves by ordinary stores)
     }
     if (warp == 1) {
         if (TWO) { tmem_alloc_pair(smem_u32(tmem_slot), Cfg::TMEM_COLS); tmem_relinquish_pair(); }
@@ -2124,7 +2124,7 @@ static int gemm_setup(const GemmCall& g, int bn, bool pair, bool int32_out, Gemm
     const uint64_t results = g.accumulate ? 1 : g.splits;
     uint64_t dc[4] = {(uint64_t)g.N, (uint64_t)g.M, results, 1};
     const uint64_t pitch = g.ldc > 0 ? g.ldc : g.N;
-    p->plain_out = pitch % 4 != 0 ? static_cast<int32_t*>(g.out) : nullptr;  // rows a tensor map cannot describe (umma_gemm_two alone)
+    p->plain_out = int32_out && pitch % 4 != 0 ? static_cast<int32_t*>(g.out) : nullptr;  // rows a tensor map cannot describe (umma_gemm_two alone)
     if (p->plain_out != nullptr) int32_out = false;
     uint64_t sc[3] = {pitch * 4, g.M * pitch * 4, results * g.M * pitch * 4};
     uint32_t bc[4] = {32, 128, 1, 1};
@@ -2158,6 +2158,7 @@ int umma_gemm(const int8_t* A, const int8_t* B, void* out, unsigned* maxabs, int
     GemmParams p{};
     const GemmCall g{A, B, out, maxabs, M, N, K, trans_a, trans_b, splits, lda, 0, ldc, 0, status};
     if (int e = gemm_setup(g, bn, pair, !fused, &m, &p)) return e;
+    if (p.plain_out != nullptr) return NITI_ERR_UNSUPPORTED;  // umma_gemm_kernel has no ordinary stores
     if (rows32 == 2) p.mma_n = 32;
     p.rows32 = rows32; p.a32 = A; p.b32 = B;
     set_fused(&p, fused);
