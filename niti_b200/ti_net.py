@@ -10,6 +10,13 @@ from .ti_loss import TiLoss
 from .ti_torch import RangeEstimate, TiDropout, TiFloatToInt8, TiLinear, TiVocabHead, exp_tensor
 
 
+def _walk_back(layers, err):
+    """The error through the layers, last first; a block without a backward of its own (torch.nn.Sequential) layer by layer."""
+    for layer in reversed(layers):
+        err = layer.backward(err) if hasattr(layer, 'backward') else _walk_back(layer, err)
+    return err
+
+
 class TiNet(Module):
     """Integer network: quantise the float input, run the layers on (int8, exponent) tuples, and
     back-propagate the integer error layer by layer -- no autograd (ti_net.py:17-32)."""
@@ -43,11 +50,7 @@ class TiNet(Module):
     def backward(self, target):
         x = self.loss(self.out, self.out_exp, target)
         for layer in reversed(self.forward_layers):
-            if isinstance(layer, torch.nn.Sequential):
-                for block in reversed(layer):
-                    x = block.backward(x)
-            else:
-                x = layer.backward(x)
+            x = _walk_back(layer, x) if isinstance(layer, torch.nn.Sequential) else layer.backward(x)
 
     def vocab_head(self):
         """The last layer if it is a TiVocabHead, else None."""
@@ -69,8 +72,7 @@ class TiNet(Module):
         head, h = self.vocab_head(), self._vocab_body(x)
         loss, e = head.distill_step(h, target[:3], *target[3:]) if isinstance(target, tuple) else head.train_step(h, target)
         self.out, self.out_exp = loss, e[1]
-        for l in reversed(list(self.forward_layers)[:-1]):
-            e = l.backward(e)
+        _walk_back(list(self.forward_layers)[:-1], e)
         return loss
 
     def _fusable_head(self, batch):
@@ -121,9 +123,7 @@ class TiNet(Module):
         lin.grad_int32acc, lin.grad_maxabs, lin.err_exp = g32, gm, err_exp
         if lin.grad_ready is not None:
             lin.grad_ready(lin)
-        e = (e8, err_exp)
-        for l in reversed(body):
-            e = l.backward(e)
+        _walk_back(body, (e8, err_exp))
         return self.out, self.out_exp
 
     def state_dict(self):
