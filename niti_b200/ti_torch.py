@@ -281,8 +281,9 @@ class TiVocabHead(TiLinear):
             raise RuntimeError("TiVocabHead: the global-exact data-parallel mode is not implemented")
         layer = self._rows(input)
         dev, shape = layer[0].device, input[0].shape
+        rows = layer[0].shape[0] // shape[0] if len(shape) > 1 and shape[0] else 1  # of a sample
         how = dict(bits=BITWIDTH, loss_mode=_mode(VOCAB_ROUND_METHOD), err_mode=_mode(ERROR_ROUND_METHOD), seed=RNG_SEED(dev), loss_stream=0xFFFF,
-                   err_stream=16 * self.layer_id + 1, sample_offset=SAMPLE_OFFSET * (layer[0].shape[0] // shape[0] if shape[0] else 1), g32=self.grad_buffer)
+                   err_stream=16 * self.layer_id + 1, sample_offset=SAMPLE_OFFSET * rows, g32=self.grad_buffer)
         if teacher is None:
             loss, err, err_exp, g32, g_max = ops.vocab_train(*layer, self._target(target, dev), self.ignore_index, **how)
         else:

@@ -80,3 +80,29 @@ def test_a_classifier_behind_blocks_of_layers(how, fused):
     for a, b in zip(*results):
         assert torch.equal(a, b)
     ops.check_status(DEV)
+
+
+def test_random_words_of_a_sample():
+    """Stochastic errors are keyed by a row's number in the whole batch, whether the rows come together, as positions of samples or
+    one at a time."""
+    net, _ = mlp([32], 300, 6)
+    head = net.vocab_head()
+    head.defer_update = True
+    rng = np.random.default_rng(7)
+    x, y = cu(rng.integers(-100, 101, (12, 32)).astype(np.int8)), cu(rng.integers(0, 300, 12))
+    e = ti_torch.exp_tensor(-7, DEV)
+    old = ti_torch.VOCAB_ROUND_METHOD, ti_torch.SAMPLE_OFFSET
+    ti_torch.VOCAB_ROUND_METHOD, ti_torch.SAMPLE_OFFSET = ti_torch.StoShift, 0
+    try:
+        ti_torch.set_seed(21, torch.device(DEV))
+
+        def gradient(offset, x, y):
+            ti_torch.SAMPLE_OFFSET = offset
+            head.train_step((x, e), y)
+            return head.grad_int32acc.clone()
+        whole = gradient(0, x, y)
+        assert torch.equal(whole, gradient(0, x.view(4, 3, 32), y.view(4, 3)))
+        assert torch.equal(whole, gradient(0, x[:6].view(2, 3, 32), y[:6].view(2, 3)) + gradient(2, x[6:].view(2, 3, 32), y[6:].view(2, 3)))
+        assert torch.equal(whole, sum(gradient(i, x[i], y[i]) for i in range(12)))
+    finally:
+        ti_torch.VOCAB_ROUND_METHOD, ti_torch.SAMPLE_OFFSET = old
