@@ -55,11 +55,18 @@ class Trainer:
 
     ``sample_offset``: global index of this rank's first sample (``dp.shard_range(global_batch, rank, world)[0]``);
     default ``rank * local_batch``, which is right for equal shards.  It keys the per-sample random bits.
+
+    A network that ends in a TiVocabHead trains on one int64 class a row; a teacher's logits go through
+    ``TiNet.train_step``.  ``global_exact`` is refused for it.
     """
 
     def __init__(self, model, local_batch, device, group=None, rank=0, world=1, use_graph=True, seed=0,
                  in_shape=(3, 32, 32), warmup_steps=2, keep_gradients=False, wgrad_side_stream=True,
                  global_exact=False, peer_update="auto", sample_offset=None, push_gradients="auto"):
+        head = getattr(model, "vocab_head", None)
+        vocab = head is not None and head() is not None
+        if vocab and global_exact and world > 1:
+            raise ValueError("Trainer: global_exact is not there for a network that ends in a TiVocabHead")
         self.model, self.device, self.group = model, torch.device(device), group
         self.rank, self.world, self.use_graph = rank, world, use_graph
         self.local_batch = local_batch
@@ -107,8 +114,6 @@ class Trainer:
         self.t = torch.zeros((local_batch,), dtype=torch.int64, device=self.device)
         # two result slots, used alternately: step i's logits stay readable while step i+1 writes the other slot.  A network that
         # ends in a TiVocabHead hands back its rows' losses, and beside them the exponent of the error that it trained on.
-        head = getattr(model, "vocab_head", None)
-        vocab = head is not None and head() is not None
         out_shape, out_type = ((local_batch,), torch.float32) if vocab else ((local_batch, self.layers[-1].weight.shape[0]), torch.int8)
         self._out_hosts = [torch.zeros(out_shape, dtype=out_type).pin_memory() for _ in range(2)]
         self._exp_hosts = [torch.zeros((), dtype=torch.int32).pin_memory() for _ in range(2)]

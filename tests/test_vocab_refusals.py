@@ -1,0 +1,18 @@
+"""What a network that ends in a vocabulary of classes, or does not, is refused before anything is set up."""
+import pytest
+
+
+def test_trainer_refuses_the_global_exact_mode():
+    from niti_b200 import ti_torch
+    from niti_b200.trainer import Trainer
+
+    class Net:
+        def vocab_head(self):
+            return object()
+
+        def weighted_layers(self):
+            raise AssertionError("the trainer went on")
+    before = ti_torch.GLOBAL_MAX_GROUP
+    with pytest.raises(ValueError, match="global_exact"):
+        Trainer(Net(), 4, "cpu", rank=0, world=2, global_exact=True)
+    assert ti_torch.GLOBAL_MAX_GROUP is before
