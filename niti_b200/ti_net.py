@@ -65,7 +65,10 @@ class TiNet(Module):
 
     def losses(self, x, target):
         """A TiVocabHead network's loss of every row, without training; ``target`` as in train_step."""
-        head, h = self.vocab_head(), self._vocab_body(x)
+        head = self.vocab_head()
+        if head is None:
+            raise RuntimeError("TiNet.losses: the network does not end in a TiVocabHead")
+        h = self._vocab_body(x)
         return head.distill_loss(h, target[:3], *target[3:]) if isinstance(target, tuple) else head.loss(h, target)
 
     def _vocab_step(self, x, target):
