@@ -13,7 +13,8 @@
 //           L = sum_c (S_c q) >> (10 + I),  q >> I being E(M - m_c)           (2^44 is 1; for the loss)
 //   loss  = (M - a_y) 2^e + ln(L 2^-44)                                       (double, stored as float32)
 //   p     = hi32(E(M - a) R) >> (n - 3),  R = (2^63 - 1) / (S >> n), 2^31 <= S >> n < 2^32    (2^30 is 1; S >= 2^34, so n >= 3)
-//   err   = p - target share, narrowed by 23 bits to int8 (2^-7), NITI's roundings
+//   err   = p - target share, narrowed by 23 bits to int8 (2^-7), NITI's roundings (pseudo-stochastically, by p's own low bits,
+//           equal classes are rounded alike)
 //
 // E ends at 2^-30, so S loses up to 2^-30 of each class of a piece far below the maximum: p is up to V 2^-30 (2.4e-4 for 2^18 classes) of
 // itself too large, a thirtieth of err's unit.  As a loss that would be all there is where one class stands alone (16 nats above 131072

@@ -439,9 +439,10 @@ def vocab_train(x, exp_x, w, exp_w, target, ignore_index=-100, *, bits=7, loss_m
     """vocab_loss and the gradients of the sum of its losses: (loss float32 [tokens], e8 int8 [tokens, features], exp_err,
     g32 int32 [classes, features], max|g32|).  (e8, exp_err) is the error of x; g32, the weight gradient in units of
     2^(exp_x - 7), is what ops.update takes; a g32 that is given receives it.  loss_mode narrows the errors of the logits to int8
-    (units of 2^-7; rounding to nearest drops every probability below 2^-8, pseudo-stochastic below 2^-19), err_mode the error of
-    x.  Stochastic modes draw from the seed's streams loss_stream (round_up(classes, 4) words a token) and err_stream.  Rows
-    without a loss have no error."""
+    (units of 2^-7): rounding to nearest drops every probability below 2^-8, pseudo-stochastic every one below 2^-19; above, that one
+    rounds by the probability's own low bits, equal probabilities alike (of a row of 2048 equal classes it drops all, of 2056 none:
+    each counts as 2^-7); stochastic is right on average.  err_mode narrows the error of x.  Stochastic modes draw from the seed's
+    streams loss_stream (round_up(classes, 4) words a token) and err_stream.  Rows without a loss have no error."""
     return _vocab(True, x, w, target, x, exp_x, w, exp_w, target, ignore_index, None, None, 0, True, bits, loss_mode, err_mode, seed,
                   loss_stream, err_stream, sample_offset, g32)
 

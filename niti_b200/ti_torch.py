@@ -234,8 +234,12 @@ class TiLinear(UpdateWeight):
 
 class TiVocabHead(TiLinear):
     """A last layer whose classes are a vocabulary: TiLinear, TiLoss and TiLinear.backward (:241-266, ti_loss.py:6-36) in one call
-    that never holds the logits, with a softmax of 30 bits (TiLoss has 11: 2048 equal classes have no error).  Rows are tokens; leading
-    dimensions (batch, position) are taken together.  No counterpart in the reference, whose networks end in 10 classes.
+    that never holds the logits, with a softmax of 30 bits (TiLoss has 11).  Rows are tokens; leading dimensions (batch, position) are
+    taken together (the other layers take rows alone).  No counterpart in the reference, whose networks end in 10 classes.
+
+    Errors are narrowed to int8 by ``VOCAB_ROUND_METHOD``.  Its default, PstoShift, takes its random bits from the probabilities
+    themselves: classes of EQUAL logits, as all of a row of zeros have, are rounded the same way, mostly to nothing.  Such a row
+    teaches its wanted class and takes nothing from the others; where rows like that matter, StoShift gives every class its share.
 
     ``forward`` and ``backward`` are TiLinear's, for the few tokens whose logits are wanted.  Rows whose target is ``ignore_index``
     have neither loss nor error; a target outside the vocabulary makes its row's loss NaN."""
@@ -595,7 +599,8 @@ ERROR_ROUND_METHOD = RoundShift
 
 GRAD_ROUND_METHOD = PstoShift
 # Errors of a vocabulary's logits, which are mostly far below half of int8's unit of 2^-7: RoundShift would drop all of them below
-# 2^-8, PstoShift those below 2^-19, StoShift none (at 20 instructions of random words a logit).
+# 2^-8, PstoShift those below 2^-19 and, above, equal ones all alike (2048 equal classes: all; 2056: none, each then 16 times too
+# large), StoShift none (at 20 instructions of random words a logit).
 VOCAB_ROUND_METHOD = PstoShift
 WEIGHT_INIT_METHOD = UniformWeights
 
