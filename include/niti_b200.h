@@ -498,8 +498,8 @@ NITI_API int niti_fc_head_train_i8(const niti_fc_head_args* args, void* stream);
 
 /* ---------------------------------------------------------------- a vocabulary of classes
  * TiLinear.forward + TiLoss.forward + TiLinear.backward (ti_torch.py:241-266, ti_loss.py:6-36) for a last layer with so many
- * classes that its logits should not be kept: the vocabulary is taken in pieces and only the wanted classes' logits, a maximum
- * and a sum per 64 classes and (for training) a bounded piece of int8 errors pass through scratch.  The softmax works on the
+ * classes that its logits should not be kept: the vocabulary is taken in pieces and (beyond a few tokens) only the wanted classes'
+ * logits, a maximum and a sum per 64 classes and (for training) a bounded piece of int8 errors pass through scratch.  The softmax works on the
  * int32 accumulators, not on logits narrowed to int8, and has 30 bits instead of TiLoss' 11.  Integers throughout, in a fixed
  * definition (vocab_kernels.cu), so results do not depend on how the work is split.  Accuracy: a cross entropy to its rounding, 6e-6
  * of what the other classes add to it and 1.2e-7; p to 6e-6 and V 2^-30 of itself (up to 2.4e-4; errors are in units of 7.8e-3).
@@ -517,9 +517,10 @@ NITI_API int niti_fc_head_train_i8(const niti_fc_head_args* args, void* stream);
  *     err_calc does (ti_torch.py:119-133), *exp_err = shift + *exp_w - 7 + temperature_log2;
  *   g32 [V][F] = err8^T x, *grad_maxabs = max |g32|, for niti_update_i8.
  *   sample_offset: global index of the first row, for the random words.
- * scratch: niti_vocab_scratch_bytes(T, F, V, entries, g32 != null) bytes, 16-byte aligned, contents irrelevant.  T, F < 2^17,
- * V <= 2^18, entries <= 128 (niti_vocab_supported), any F (rows of other lengths than multiples of 16 go through copies).  x, w,
- * e8 and g32 16-byte aligned.  Calls on different streams need scratch of their own. */
+ * scratch: niti_vocab_scratch_bytes(T, F, V, entries, g32 != null) bytes, 16-byte aligned, contents irrelevant.  What makes it large:
+ * 8 T ceil(V / 64) bytes of statistics; in training errors of up to 96 MB and 4 T round_up(F, 4) bytes, but up to four tokens (that fit
+ * into shared memory) keep all their logits instead, 4 T V bytes; where there are more, rows of F that are no multiple of 16 go through
+ * copies of x and of the whole of w, (T + V) round_up(F, 16) bytes.  T, F < 2^17, V <= 2^18, entries <= 128 (niti_vocab_supported).  x, w, e8 and g32 16-byte aligned.  Calls on different streams need scratch of their own. */
 typedef struct niti_vocab_args {
     const int8_t* x; const int32_t* exp_x;
     const int8_t* w; const int32_t* exp_w;

@@ -908,8 +908,7 @@ __global__ void __launch_bounds__(256) vocab_patch_kernel(const int* entries, lo
 }
 
 // ---------------------------------------------------------------------------------------------- a few tokens' way back
-// Both products that lead back for the tokens of vocab_thin_kernel, from the logits it kept (no more bytes than a sixteenth of w's
-// features): w read once, the gradient written once, which is nearly all there is to do (an outer product of a few rows).  A thread
+// Both products that lead back for the tokens of vocab_thin_kernel, from the logits it kept (4 T / F of w's bytes): w read once, the gradient written once, which is nearly all there is to do (an outer product of a few rows).  A thread
 // owns four features and sixteen classes of a batch, whose w it fetches at once (stores in between would hold the later ones back);
 // their errors with the features' tokens (dp4a over tokens) are the gradient, which leaves at once; with w (dp4a over classes) they add
 // up to the features' error, which is added to e32 at the end.  Rows shorter than 1024 features leave room for several groups of

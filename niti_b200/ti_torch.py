@@ -234,7 +234,7 @@ class TiLinear(UpdateWeight):
 
 class TiVocabHead(TiLinear):
     """A last layer whose classes are a vocabulary: TiLinear, TiLoss and TiLinear.backward (:241-266, ti_loss.py:6-36) in one call
-    that never holds the logits, with a softmax of 30 bits (TiLoss has 11).  Rows are tokens; leading dimensions (batch, position) are
+    that writes no logits out, with a softmax of 30 bits (TiLoss has 11).  Rows are tokens; leading dimensions (batch, position) are
     taken together (the other layers take rows alone).  No counterpart in the reference, whose networks end in 10 classes.
 
     Errors are narrowed to int8 by ``VOCAB_ROUND_METHOD``.  Its default, PstoShift, takes its random bits from the probabilities
